@@ -27,6 +27,10 @@ KIND_RBOX = 0
 KIND_POLY = 1
 KIND_HBB = 2   # NMS only: x1, y1, x2, y2 (+ score) with the reference's +1 convention
 MODE = {'iou': 0, 'iof': 1}
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # OBB_F32 / OBB_BF16 / OBB_F16
+ACTS = {'none': 0, 'relu': 1, 'gelu': 2, 'silu': 3}                   # OBB_ACT_*
+LINEAR_FORWARD, LINEAR_ACT_BACKWARD, LINEAR_BACKWARD_INPUT, LINEAR_BACKWARD_WEIGHT = range(4)
+DISTILL_MAX_K = 1024    # OBB_DISTILL_MAX_K
 NMS_STRICT = 1          # OBB_NMS_STRICT: suppress on `>` (nms_kernel.cu:61) instead of `>=` (nms_cpu.cpp:56)
 NMS_RETAIN = 2          # OBB_NMS_RETAIN: the workspace is the caller's alone from call to call -- three launches instead of four (obbops.h)
 NMS_RESULT_BYTES = 64   # OBB_NMS_RESULT_BYTES
@@ -188,6 +192,21 @@ def lib():
         L.obb_tiled_merge_f32.restype = i32
         L.obb_tiled_result.argtypes = [vp, i32, i64, i32, i32, i64, ctypes.c_size_t, ctypes.POINTER(i64)]
         L.obb_tiled_result.restype = i32
+        sz = ctypes.c_size_t
+        L.obb_linear_workspace_bytes.argtypes = [i64, i64, i64, i32, i32]
+        L.obb_linear_workspace_bytes.restype = sz
+        L.obb_linear_forward.argtypes = [vp, i64, vp, i64, vp, vp, i64, i64, i64, i64, i32, i32, vp, vp, vp, sz, vp]
+        L.obb_linear_forward.restype = i32
+        L.obb_linear_act_backward.argtypes = [vp, vp, vp, i64, i64, i32, i32, vp, vp, vp, sz, vp]
+        L.obb_linear_act_backward.restype = i32
+        L.obb_linear_backward_input.argtypes = [vp, vp, i64, i64, i64, i64, i32, vp, vp, sz, vp]
+        L.obb_linear_backward_input.restype = i32
+        L.obb_linear_backward_weight.argtypes = [vp, vp, i64, i64, i64, i64, i32, vp, vp, sz, vp]
+        L.obb_linear_backward_weight.restype = i32
+        L.obb_topk_distill_forward.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, i32, i32, f32, vp, vp, vp, f32, vp, vp]
+        L.obb_topk_distill_forward.restype = i32
+        L.obb_topk_distill_backward.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, i32, i32, f32, vp, vp, vp, i64, f32, vp, i64, vp]
+        L.obb_topk_distill_backward.restype = i32
         _lib = L
     return _lib
 

@@ -631,6 +631,73 @@ OBB_API int obb_roi_backward_gather_nhwc_f32(const float *grad_out_dev, int B, i
                                              void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Fused linear layer: a matrix product with bias, residual and activation in its epilogue, and its gradients.
+ *   z = x w^T + bias + res,  y = act(z);   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum_m dz,  dres = dz
+ * x (m, k) with row pitch ldx, w (n, k) with row pitch ldw, bias (n) or NULL, res (m, n) with row pitch ldr (0 = one row
+ * for all) or NULL, y (m, n); all of one dtype (pitches in elements), products and sums in fp32, one rounding to the
+ * dtype at the end.  Any sizes (zero too), pitches and element-aligned pointers; outputs must not overlap inputs.
+ * Training: gelu and silu need the pre-activation, written to z (m, n) fp32 (NULL otherwise); relu needs y only.
+ *   obb_linear_act_backward    dy (m, n) -> dz (m, n) of the dtype (NULL: not wanted; may be dy itself), dbias (n) (NULL: not wanted)
+ *   obb_linear_backward_input  dz, w -> dx (m, k)          obb_linear_backward_weight  dz, x -> dw (n, k)
+ * Deterministic: no atomics, fixed order of the sums.  Each call's workspace is obb_linear_workspace_bytes(m, n, k,
+ * dtype, op) bytes (16-byte aligned; contents need not be kept, 0 bytes: may be NULL); calls that run at the same time
+ * need a workspace each.
+ * Replaces: the FC layers of ConvFCBBoxHead (mmdet/models/bbox_heads/convfc_bbox_head.py:175-188: nn.Linear + ReLU) and
+ *           of RBBoxHead (rbbox_head.py:157-195); on channels-last maps the 1 x 1 convolutions of the bottlenecks with
+ *           their shortcut and ReLU (backbones/resnet.py:101-125) and of the FPN laterals (necks/fpn.py:138-178).
+ * ------------------------------------------------------------------------- */
+#define OBB_F32 0
+#define OBB_BF16 1
+#define OBB_F16 2
+#define OBB_ACT_NONE 0
+#define OBB_ACT_RELU 1
+#define OBB_ACT_GELU 2   /* z Phi(z), by erf */
+#define OBB_ACT_SILU 3   /* z / (1 + exp(-z)) */
+#define OBB_LINEAR_FORWARD 0
+#define OBB_LINEAR_ACT_BACKWARD 1
+#define OBB_LINEAR_BACKWARD_INPUT 2
+#define OBB_LINEAR_BACKWARD_WEIGHT 3
+OBB_API size_t obb_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype, int op);
+OBB_API int obb_linear_forward(const void *x_dev, int64_t ldx, const void *w_dev, int64_t ldw, const void *bias_dev,
+                               const void *res_dev, int64_t ldr, int64_t m, int64_t n, int64_t k, int dtype, int act,
+                               void *y_dev, float *z_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+OBB_API int obb_linear_act_backward(const void *dy_dev, const void *y_dev, const float *z_dev, int64_t m, int64_t n, int dtype,
+                                    int act, void *dz_dev, void *dbias_dev, void *workspace_dev, size_t workspace_bytes,
+                                    void *stream);
+OBB_API int obb_linear_backward_input(const void *dz_dev, const void *w_dev, int64_t ldw, int64_t m, int64_t n, int64_t k,
+                                      int dtype, void *dx_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+OBB_API int obb_linear_backward_weight(const void *dz_dev, const void *x_dev, int64_t ldx, int64_t m, int64_t n, int64_t k,
+                                       int dtype, void *dw_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Distillation of class logits from a teacher's top logits.  Row r: logits s (classes, row pitch ld), k teacher entries
+ * (value, index); an entry whose index lies outside [0, classes) is absent.
+ *   p = softmax(values / T) over the entries present,  q = softmax(s / T) over all classes
+ *   row_loss = weight T^2 sum_j p_j (log p_j - log q[index_j]),  loss = scale * sum of row_loss (fixed order)
+ *   dlogits[v] = grad scale weight T (q[v] - sum of p_j with index_j = v)
+ * A row without an entry (none present, or all of them -inf) and a row of weight 0 have loss 0 and gradient 0 whatever
+ * their logits hold; an index that comes twice counts twice.  p_j = 0 adds nothing (also where q is 0); logits of -inf have
+ * q = 0.  No gradient reaches the teacher.
+ *   dtype / vtype     OBB_F32 / OBB_BF16 / OBB_F16 of logits (and dlogits) / of the teacher's values; index_bytes 4 or 8
+ *   weight_dev        (rows) fp32, or NULL = 1;   k <= OBB_DISTILL_MAX_K
+ *   row_loss_dev      (rows) fp32;   stats_dev (rows, 2) fp32, what the backward needs (NULL: no backward follows)
+ *   loss_dev          one fp32, or NULL: only the rows' losses are wanted
+ *   grad_dev          grad_stride 0: one fp32 (of loss; `scale` as in the forward), 1: (rows) fp32 (of row_loss; scale 1)
+ * Replaces: nothing of the reference (its heads train on hard labels); stands beside rbbox_target
+ *           (mmdet/core/rbbox/rbbox_target.py:8-93), whose label_weights are its `weight`.
+ * ------------------------------------------------------------------------- */
+#define OBB_DISTILL_MAX_K 1024
+OBB_API int obb_topk_distill_forward(const void *logits_dev, int64_t ld, int64_t rows, int64_t classes, int dtype,
+                                     const void *values_dev, const void *indices_dev, int k, int vtype, int index_bytes,
+                                     float temperature, const float *weight_dev, float *row_loss_dev, float *stats_dev,
+                                     float scale, float *loss_dev, void *stream);
+OBB_API int obb_topk_distill_backward(const void *logits_dev, int64_t ld, int64_t rows, int64_t classes, int dtype,
+                                      const void *values_dev, const void *indices_dev, int k, int vtype, int index_bytes,
+                                      float temperature, const float *weight_dev, const float *stats_dev,
+                                      const float *grad_dev, int64_t grad_stride, float scale, void *dlogits_dev, int64_t ldd,
+                                      void *stream);
+
+/* ---------------------------------------------------------------------------
  * Test / tuning hooks.  NOT part of the drop-in surface (no reference counterpart): the
  * parity tests use them to force every size through every code path, and the experiment
  * scripts under tools/ to sweep launch geometry.  Process-wide; value < 0 restores the

@@ -1,0 +1,447 @@
+"""Fused linear layer (aidet_amd.linear, obb_linear_*): refusals on the CPU, values and gradients on the GPU against a
+plain implementation in 64 bits.
+
+Tolerances.  u = 2^-24 is half a step of fp32; half a step of the output's type is eps / 2 relative.
+* A sum of K products kept in fp32 makes at most K roundings of at most u times a partial sum; partial sums of terms with
+  independent signs have the size s = sqrt(sum of the squared terms), and the roundings are independent too: their sum has
+  a deviation below sqrt(K) u s.  8 of those are allowed, plus 8 u of every operand of the epilogue.
+* |act'| <= 1.13 for every activation; the functions themselves are good to a few u.
+* dz is rounded to the type once before the gradients' products: another eps / 2 of every term, independent: 4 times
+  eps / 2 sqrt(sum of the squared terms).  act'' <= 0.8 brings the error of z into dz.
+"""
+import ctypes
+
+import pytest
+import torch
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+DEV = 'cuda:0'
+
+
+def act64(z, act):
+    if act == 'relu':
+        return z.clamp(min=0)
+    if act == 'gelu':
+        return 0.5 * z * torch.erfc(-z / 2 ** 0.5)
+    if act == 'silu':
+        return z * torch.sigmoid(z)
+    return z
+
+
+def slope64(z, act):
+    if act == 'relu':
+        return (z > 0).double()
+    if act == 'gelu':
+        return 0.5 * torch.erfc(-z / 2 ** 0.5) + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    if act == 'silu':
+        s = torch.sigmoid(z)
+        return s * (1 + z * (1 - s))
+    return torch.ones_like(z)
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def product64(a, b):
+    """a (M, K) @ b (K, N) in 64 bits, and the deviation's unit: sqrt of the sum of the squared terms."""
+    a, b = a.double(), b.double()
+    return a @ b, ((a * a) @ (b * b)).sqrt()
+
+
+def summed(s, terms, more):
+    """allowed error of fp32 sums of `terms` products, `more` = epilogue operands' size"""
+    return 8 * (terms + 8) ** 0.5 * U * s + 8 * U * more
+
+
+def tiny(t):
+    return 2 * torch.finfo(t).tiny if t != torch.float16 else 2.0 ** -24     # (fp16: values below its normal range step by 2^-24)
+
+
+def make(m, k, n, dtype, bias, residual, seed=0, pad=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn(m, k + pad, generator=g, device=DEV).to(dtype)[:, :k]
+    w = (torch.randn(n, k, generator=g, device=DEV) * max(k, 1) ** -0.5).to(dtype)
+    b = torch.randn(n, generator=g, device=DEV).to(dtype) if bias else None
+    r = torch.randn(m, n, generator=g, device=DEV).to(dtype) if residual else None
+    return x, w, b, r
+
+
+def reference(x, w, b, r, act):
+    """(y64, z64, allowed error of z, of y)"""
+    z, s = product64(x, w.t())
+    more = z.abs()
+    for t in (b, r):
+        if t is not None:
+            z = z + t.double()
+            more = more + t.double().abs()
+    ez = summed(s, x.size(1), more)
+    y = act64(z, act)
+    return y, z, ez, 1.13 * ez + 4 * U * (y.abs() + z.abs()) + half_step(x.dtype) * y.abs() + tiny(x.dtype)
+
+
+def check(x, w, b, r, act):
+    from aidet_amd import fused_linear
+    got = fused_linear(x, w, b, r, act)
+    want, _, _, tol = reference(x.reshape(-1, x.size(-1)), w, b, None if r is None else r.reshape(-1, w.size(0)), act)
+    assert got.dtype == x.dtype and got.shape == x.shape[:-1] + (w.size(0), )
+    off = (got.reshape(want.shape).double() - want).abs() - tol
+    assert bool((off <= 0).all()), (float(off.max()), int(off.argmax()))
+    return got
+
+
+# ---- refusals and host logic: no GPU ------------------------------------------------------------------------------------
+def test_refuses_what_it_cannot_serve():
+    from aidet_amd import FusedLinear, fused_linear
+    x, w = torch.zeros(3, 4), torch.zeros(5, 4)
+    with pytest.raises(TypeError):
+        fused_linear([[1.]], w)
+    with pytest.raises(NotImplementedError):
+        fused_linear(x, w)
+    with pytest.raises(ValueError):
+        FusedLinear(4, 5, act='tanh')
+    m = FusedLinear(4, 5, act='silu')
+    assert set(m.state_dict()) == {'weight', 'bias'} and 'act=silu' in repr(m)
+    m.load_state_dict(torch.nn.Linear(4, 5).state_dict())
+
+
+class _Cuda(torch.Tensor):
+    """a CPU tensor that says it is on the GPU: what the wrapper checks before any device work"""
+    is_cuda = True
+
+
+def _fake(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_Cuda)
+
+
+@pytest.mark.parametrize('args, error', [
+    ((_fake(3, 4), _fake(5, 4, dtype=torch.float16)), TypeError),
+    ((_fake(3, 4, dtype=torch.float64), _fake(5, 4, dtype=torch.float64)), TypeError),
+    ((_fake(3, 4), _fake(5, 3)), ValueError),
+    ((_fake(3, 4), _fake(5, 4, 1)), ValueError),
+    ((_fake(3, 4), _fake(5, 4), _fake(4)), ValueError),
+    ((_fake(3, 4), _fake(5, 4), _fake(5, 1)), ValueError),
+    ((_fake(3, 4), _fake(5, 4), None, _fake(1, 5)), ValueError),
+    ((_fake(3, 4), _fake(5, 4), None, None, 'tanh'), ValueError),
+    ((_fake(3, 4), _fake(5, 4), torch.zeros(5)), NotImplementedError),
+])
+def test_wrapper_refusals(args, error):
+    from aidet_amd import fused_linear
+    with pytest.raises(error):
+        fused_linear(*args)
+
+
+def test_c_abi_refusals_without_gpu():
+    from aidet_amd import _lib
+    L = _lib.lib()
+    one, null = ctypes.c_void_p(256), None     # (never dereferenced: validation fails first)
+    f = L.obb_linear_forward
+    assert f(one, 4, one, 4, null, null, 0, -1, 5, 4, 0, 0, one, null, null, 0, null) == _lib.OBB_EINVAL
+    assert f(one, 4, one, 4, null, null, 0, 3, 5, 4, 9, 0, one, null, null, 0, null) == _lib.OBB_EINVAL
+    assert f(one, 4, one, 4, null, null, 0, 3, 5, 4, 0, 7, one, null, null, 0, null) == _lib.OBB_EINVAL
+    assert b'activation' in L.obb_last_error()
+    assert f(one, 3, one, 4, null, null, 0, 3, 5, 4, 0, 0, one, null, null, 0, null) == _lib.OBB_EINVAL
+    assert f(one, 4, one, 4, null, one, 3, 3, 5, 4, 0, 0, one, null, null, 0, null) == _lib.OBB_EINVAL
+    assert b'pitch' in L.obb_last_error()
+    assert f(null, 4, one, 4, null, null, 0, 3, 5, 4, 0, 0, one, null, null, 0, null) == _lib.OBB_EINVAL
+    assert f(null, 4, null, 4, null, null, 0, 0, 5, 4, 0, 0, null, null, null, 0, null) == _lib.OBB_OK
+    assert L.obb_linear_act_backward(one, null, null, 3, 5, 0, 1, one, null, null, 0, null) == _lib.OBB_EINVAL    # relu: no y
+    assert L.obb_linear_act_backward(one, one, null, 3, 5, 0, 2, one, null, null, 0, null) == _lib.OBB_EINVAL     # gelu: no z
+    assert L.obb_linear_act_backward(one, one, one, 3, 5, 0, 1, null, null, null, 0, null) == _lib.OBB_EINVAL
+    assert L.obb_linear_act_backward(one, one, one, 3, 5, 0, 1, one, one, null, 0, null) == _lib.OBB_EWORKSPACE
+    assert L.obb_linear_backward_input(one, one, 3, 3, 5, 4, 0, one, null, 0, null) == _lib.OBB_EINVAL
+    assert L.obb_linear_backward_weight(one, null, 4, 3, 5, 4, 0, one, null, 0, null) == _lib.OBB_EINVAL
+    assert L.obb_linear_backward_weight(one, one, 4, 3, 5, 4, 3, one, null, 0, null) == _lib.OBB_EINVAL
+    assert L.obb_linear_workspace_bytes(-1, 5, 4, 0, 0) == 0
+
+
+# ---- values --------------------------------------------------------------------------------------------------------------
+SIZES = [(1, 1, 1), (1, 64, 64), (2, 7, 3), (17, 33, 65), (64, 64, 64), (1, 4096, 1000), (5, 1024, 16), (63, 129, 257), (128, 256, 128),
+         (200, 1000, 80), (257, 512, 255), (1000, 72, 40), (300, 2056, 520), (4097, 24, 8), (33, 12544, 96)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m, k, n', SIZES)
+def test_forward_sizes(m, k, n, dtype):
+    x, w, b, r = make(m, k, n, dtype, True, True, seed=m + k + n)
+    check(x, w, b, r, 'relu')
+    check(x, w, None, None, 'none')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('act', ['none', 'relu', 'gelu', 'silu'])
+@pytest.mark.parametrize('bias, residual', [(False, False), (True, False), (False, True), (True, True)])
+def test_forward_epilogue(act, bias, residual, dtype):
+    x, w, b, r = make(150, 200, 136, dtype, bias, residual, seed=3)
+    check(x, w, b, r, act)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m, n', [(3, 512), (300, 256)])
+def test_forward_layouts(m, n, dtype):
+    """rows of a wider buffer, unaligned starts, transposed storage, leading dimensions, an expanded residual"""
+    k = 320
+    x, w, b, r = make(m, k, n, dtype, True, True, seed=5)
+    want = check(x, w, b, r, 'silu')
+    from aidet_amd import fused_linear
+    for pad, start in ((8, 0), (8, 8), (1, 0), (5, 3), (3, 1)):
+        wide = torch.full((m, k + start + pad), float('nan'), dtype=dtype, device=DEV)
+        wide[:, start:start + k] = x
+        wide_w = torch.full((n, k + start + pad), float('nan'), dtype=dtype, device=DEV)
+        wide_w[:, start:start + k] = w
+        wide_r = torch.full((m, n + start + pad), float('nan'), dtype=dtype, device=DEV)
+        wide_r[:, start:start + n] = r
+        got = check(wide[:, start:start + k], wide_w[:, start:start + k], b, wide_r[:, start:start + n], 'silu')
+        assert got.is_contiguous()
+    assert torch.equal(fused_linear(x.t().contiguous().t(), w.t().contiguous().t(), b, r, 'silu'), want)
+    assert torch.equal(fused_linear(x.view(1, m, k), w, b, r.view(1, m, n), 'silu'), want[None])
+    row = r[:1].expand(m, n)
+    assert torch.equal(fused_linear(x, w, b, row, 'silu'), fused_linear(x, w, b, row.contiguous(), 'silu'))
+    one = fused_linear(x[0], w, b, r[0], 'silu')
+    assert one.shape == (n, ) and torch.equal(one, fused_linear(x[:1], w, b, r[:1], 'silu')[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_empty_sizes(dtype):
+    from aidet_amd import fused_linear
+    x, w, b, r = make(0, 8, 5, dtype, True, True)
+    assert fused_linear(x, w, b, r, 'relu').shape == (0, 5)
+    x, w, b, r = make(4, 0, 5, dtype, True, True)
+    assert torch.equal(fused_linear(x, w, b, r, 'none'), (b.float() + r.float()).to(dtype))
+    x, w, b, r = make(4, 8, 0, dtype, True, True)
+    assert fused_linear(x, w, b, r, 'relu').shape == (4, 0)
+    # gradients of an empty batch: zeros for what is there
+    x, w, b, _ = make(0, 8, 5, dtype, True, False)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(fused_linear(*leaves, act='gelu').float().sum(), leaves)
+    assert dx.shape == (0, 8) and not dw.any() and not db.any() and dw.shape == w.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m', [2, 150])
+def test_infinities_and_nans_stay_in_their_rows(m, dtype):
+    """IEEE: an infinite or NaN input reaches its row's (weight: its column's) outputs and no other"""
+    from aidet_amd import fused_linear
+    k, n = 264, 200
+    x, w, b, _ = make(m, k, n, dtype, True, False, seed=8)
+    clean = fused_linear(x, w, b)
+    x2, w2 = x.clone(), w.clone()
+    x2[1, 5] = float('inf')
+    w2[7] = 0
+    got = fused_linear(x2, w2, b)
+    want = x2.double() @ w2.double().t() + b.double()     # (+-inf by the weight's sign; NaN at the zero weights)
+    assert torch.equal(got[1].isnan(), want[1].isnan()) and torch.equal(got[1].isinf(), want[1].isinf())
+    assert torch.equal(got[1][got[1].isinf()].double(), want[1][want[1].isinf()])
+    others = [c for c in range(n) if c != 7]
+    assert torch.equal(got[0][others], clean[0][others]) and bool((got[0, 7] == b[7]))
+    x2[1, 5] = float('nan')
+    got = fused_linear(x2, w, b)
+    assert bool(got[1].isnan().all()) and torch.equal(got[0], clean[0])
+    w2 = w.clone()
+    w2[3, 2] = -float('inf')
+    got = fused_linear(x, w2, b)
+    assert bool(got[:, 3].isinf().all()) and torch.equal(got[:, 4:], clean[:, 4:])
+    assert torch.equal(got[:, 3] > 0, x[:, 2] < 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('m', [1, 130])
+@pytest.mark.parametrize('size', [2.0 ** 60, 2.0 ** -60])
+def test_fp32_keeps_its_range(m, size):
+    """products of very large and very small factors: relative accuracy as at 1"""
+    x, w, b, _ = make(m, 500, 140, torch.float32, False, False, seed=9)
+    check(x * size, w / size, None, None, 'none')
+    check(x * size, w * min(size, 1.), None, None, 'none')
+
+
+@pytest.mark.gpu
+def test_pitches_past_32_bits():
+    """rows 2^31 and more elements apart"""
+    from aidet_amd import fused_linear
+    pitch, k = (1 << 30) + 8, 40
+    buf = torch.empty(4 * pitch, dtype=torch.bfloat16, device=DEV)
+    x, w, b, _ = make(4, k, 130, torch.bfloat16, True, False, seed=10)
+    far = buf.as_strided((4, k), (pitch, 1))
+    far.copy_(x)
+    assert torch.equal(fused_linear(far, w, b, act='relu'), fused_linear(x, w, b, act='relu'))
+    x, w, b, _ = make(130, k, 4, torch.bfloat16, True, False, seed=11)
+    far.copy_(w)
+    assert torch.equal(fused_linear(x, far, b, act='relu'), fused_linear(x, w, b, act='relu'))
+
+
+# ---- gradients -----------------------------------------------------------------------------------------------------------
+def gradients(x, w, b, r, act, dy):
+    from aidet_amd import fused_linear
+    leaves = [t.detach().requires_grad_(True) for t in (x, w, b, r) if t is not None]
+    it = iter(leaves)
+    args = [None if t is None else next(it) for t in (x, w, b, r)]
+    return torch.autograd.grad(fused_linear(*args, act=act), leaves, dy)
+
+
+def check_gradients(x, w, b, r, act, dy):
+    dtype = x.dtype
+    h = half_step(dtype)
+    got = list(gradients(x, w, b, r, act, dy))
+    _, z, ez, _ = reference(x, w, b, r, act)
+    dz = dy.double() * slope64(z, act)
+    edz = dy.double().abs() * (0.8 * ez + 8 * U) + h * dz.abs() + tiny(dtype)      # per element, independent of each other
+
+    def product(a, ea, c):            # (a +- ea) @ c
+        p, s = product64(a, c)
+        spread = 4 * ((ea * ea) @ (c.double() ** 2)).sqrt()
+        return p, summed(s, a.size(1), p.abs()) + spread + h * p.abs() + tiny(dtype)
+    want = [product(dz, edz, w), product(dz.t(), edz.t(), x)]
+    if b is not None:
+        want.append((dz.sum(0), summed((dz * dz).sum(0).sqrt(), x.size(0), dz.sum(0).abs()) + 4 * ((edz - h * dz.abs()) ** 2).sum(0).sqrt()
+                     + h * dz.sum(0).abs() + tiny(dtype)))
+    if r is not None:
+        want.append((dz, edz))
+    for g, (v, tol), name in zip(got, want, ['x', 'w'] + ['b'] * (b is not None) + ['r'] * (r is not None)):
+        off = (g.double() - v).abs() - tol
+        assert g.dtype == dtype and bool((off <= 0).all()), (name, float(off.max()), int(off.argmax()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m, k, n', [(1, 1, 1), (1, 200, 96), (3, 70, 33), (64, 64, 64), (65, 257, 129), (256, 512, 384), (700, 40, 24), (130, 1031, 17),
+                                     (2050, 136, 72)])
+def test_gradients_sizes(m, k, n, dtype):
+    x, w, b, r = make(m, k, n, dtype, True, True, seed=m + n)
+    dy = torch.randn(m, n, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).to(dtype)
+    check_gradients(x, w, b, r, 'silu', dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('act', ['none', 'gelu', 'silu'])
+@pytest.mark.parametrize('bias, residual', [(False, False), (True, True)])
+def test_gradients_epilogue(act, bias, residual, dtype):
+    x, w, b, r = make(140, 96, 200, dtype, bias, residual, seed=4, pad=8)
+    dy = torch.randn(140, 200, generator=torch.Generator(device=DEV).manual_seed(3), device=DEV).to(dtype)
+    check_gradients(x, w, b, r, act, dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m, k, n', [(90, 60, 130), (200, 128, 64)])
+def test_gradients_relu(m, k, n, dtype):
+    """whole numbers and a bias of a half: z is exact and never 0, so every gradient has one value -- and an exact one
+    while its sum stays below 2^24 (fp32) and within the type"""
+    g = torch.Generator(device=DEV).manual_seed(6)
+    x = torch.randint(-2, 3, (m, k), generator=g, device=DEV).to(dtype)
+    w = torch.randint(-2, 3, (n, k), generator=g, device=DEV).to(dtype)
+    b = torch.full((n, ), 0.5, device=DEV, dtype=dtype)
+    dy = torch.randint(-2, 3, (m, n), generator=g, device=DEV).to(dtype)
+    dx, dw, db = gradients(x, w, b, None, 'relu', dy)
+    dz = dy.double() * ((x.double() @ w.double().t() + 0.5) > 0)
+    for got, want in ((dx, dz @ w.double()), (dw, dz.t() @ x.double()), (db, dz.sum(0))):
+        assert torch.equal(got, want.to(dtype))
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    """fp32 against central differences of the plain form in 64 bits, gelu: (f(t + h d) - f(t - h d)) / 2h for random
+    directions d.  The difference quotient is good to ~1e-9 relative (h = 1e-5); the kernel's sums to the tolerance below:
+    a scalar product of ~1e4 terms, each within 2e-6 of its size, independent."""
+    m, k, n = 37, 50, 41
+    x, w, b, r = make(m, k, n, torch.float32, True, True, seed=12)
+    g = torch.Generator(device=DEV).manual_seed(13)
+    dy = torch.randn(m, n, generator=g, device=DEV)
+    grads = gradients(x, w, b, r, 'gelu', dy)
+    base = [t.double() for t in (x, w, b, r)]
+    for i, got in enumerate(grads):
+        d = torch.randn(base[i].shape, generator=g, device=DEV).double()
+
+        def f(h):
+            t = list(base)
+            t[i] = t[i] + h * d
+            return (dy.double() * act64(t[0] @ t[1].t() + t[2] + t[3], 'gelu')).sum()
+        want = (f(1e-5) - f(-1e-5)) / 2e-5
+        have = (got.double() * d).sum()
+        size = ((got.double() * d) ** 2).sum().sqrt()
+        assert abs(float(have - want)) <= 2e-5 * float(size) + 1e-6 * abs(float(want)), (i, float(have), float(want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_gradients_only_where_wanted_and_broadcast(dtype):
+    from aidet_amd import fused_linear
+    x, w, b, _ = make(50, 64, 40, dtype, True, False, seed=14)
+    row = torch.randn(40, device=DEV).to(dtype).requires_grad_(True)
+    w.requires_grad_(True)
+    y = fused_linear(x, w, b, row.expand(50, 40), 'none')
+    dw, dr = torch.autograd.grad(y.float().sum(), (w, row))       # (an expanded gradient of y)
+    assert torch.equal(dr, torch.full_like(dr, 50.))
+    v, s = product64(torch.ones(40, 50, device=DEV), x)
+    assert bool(((dw.double() - v).abs() <= summed(s, 50, v.abs()) + half_step(dtype) * v.abs()).all())
+    # the same weight twice in one graph: the gradients add
+    x.requires_grad_(True)
+    sq = (torch.randn(64, 64, device=DEV) / 8).to(dtype).requires_grad_(True)
+    h = fused_linear(x, sq, act='silu')
+    both, = torch.autograd.grad(fused_linear(h, sq).float().sum(), sq, retain_graph=True)
+    assert both.shape == sq.shape and bool(both.isfinite().all())
+    with pytest.raises(RuntimeError):                             # differentiable once
+        gx, = torch.autograd.grad(h.float().sum(), x, create_graph=True)
+        gx.float().sum().backward()
+
+
+@pytest.mark.gpu
+def test_same_bits_every_run():
+    for dtype in TYPES:
+        x, w, b, r = make(700, 3000, 260, dtype, True, True, seed=15)
+        dy = torch.randn(700, 260, device=DEV).to(dtype)
+        first = gradients(x, w, b, r, 'gelu', dy)
+        for _ in range(3):
+            assert all(torch.equal(p, q) for p, q in zip(first, gradients(x, w, b, r, 'gelu', dy)))
+
+
+@pytest.mark.gpu
+def test_other_stream_and_two_at_once():
+    from aidet_amd import fused_linear
+    x, w, b, r = make(600, 2000, 300, torch.bfloat16, True, True, seed=16)
+    want = fused_linear(x, w, b, r, 'gelu')
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            outs.append([fused_linear(x, w, b, r, 'gelu') for _ in range(4)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for per in outs for o in per)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_captured_step_replays(dtype):
+    """forward + backward captured, replayed on changed inputs with eager work between: every replay the eager bits"""
+    from aidet_amd import fused_linear
+    x, w, b, r = make(90, 1100, 130, dtype, True, True, seed=17)
+    dy = torch.randn(90, 130, device=DEV).to(dtype)
+    leaves = [t.requires_grad_(True) for t in (x.contiguous(), w, b, r)]
+
+    def step():
+        y = fused_linear(*leaves, act='gelu')
+        return [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(torch.randn(90, 1100, device=DEV))
+        want = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), i
