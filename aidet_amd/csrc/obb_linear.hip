@@ -1,6 +1,8 @@
 // obb_linear.hip -- matrix product with bias, residual and activation in its epilogue, and its gradients.
 //
 //   z = x W^T + b + r,  y = act(z);   dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = sum_m dz,  dr = dz
+#include <utility>
+
 #include "obb_linear_internal.h"
 
 namespace obb {
@@ -73,9 +75,81 @@ __global__ __launch_bounds__(256) void gemm_general_kernel(Gemm<T> g, int64_t ti
       }
 }
 
+// ---- the splits of K joined: eight columns a thread, splits in order -----------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void join_splits_kernel(Gemm<T> g, const float *partial, int splits, int64_t per_row) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / per_row, n = i % per_row * 8;
+  if (m >= g.m) return;
+  Columns c;
+  c.load(g, n);
+  const bool whole = n + 8 <= g.n && (g.n & 3) == 0;
+  f32x4 lo = {}, hi = {};
+  for (int s = 0; s < splits; s++) {
+    const float *p = partial + ((int64_t)s * g.m + m) * g.n + n;
+    if (whole) {
+      lo += *(const f32x4 *)p;
+      hi += *(const f32x4 *)(p + 4);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (n + e < g.n) {
+          if (e < 4) lo[e] += p[e];
+          else hi[e - 4] += p[e];
+        }
+    }
+  }
+  epilogue8(g, c, m, n, lo, hi);
+}
+
+template <typename T>
+int join_splits(const Gemm<T> &g, const float *partial, int splits, hipStream_t stream) {
+  const int64_t per_row = (g.n + 7) / 8, blocks = (g.m * per_row + 255) / 256;
+  if (blocks > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many blocks");
+  join_splits_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(g, partial, splits, per_row);
+  OBB_LAUNCH_CHECK();
+  return OBB_OK;
+}
+
+Plan plan16(int64_t m, int64_t n, int64_t k) {
+  const int force = (int)tuning(OBB_TUNE_LINEAR_TILE, 0), force_s = (int)tuning(OBB_TUNE_LINEAR_SPLITS, 0);
+  // the cheapest of the tiles and splits by the time of a slab (64 k) of one workgroup, the rounds the device needs, and what
+  // the splits' sums cost to write and read back
+  const int64_t slabs = (k + 63) / 64;
+  Plan best = {64, 1};
+  double least = 1e30;
+  for (int tile : {256, 128, 64}) {
+    if (force && tile != force) continue;
+    const double slab_us = tile == 256 ? 1.75 : tile == 128 ? 0.51 : 0.17;      // (of one workgroup, its share of a full device)
+    const int together = tile == 256 ? 1 : tile == 128 ? 2 : 4;
+    const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
+    for (int s = 1; s <= 16 && s <= (slabs > 1 ? slabs : 1); s *= 2) {
+      if (force_s && s != force_s) continue;
+      const int64_t rounds = (tiles * s + 256 * together - 1) / (256 * together);
+      const int64_t per_cu = (tiles * s + 255) / 256;
+      const double one = slab_us * (per_cu < together ? (per_cu < 1 ? 1 : per_cu) : together);
+      double us = rounds * ((slabs + s - 1) / s) * one + 2.0;
+      if (s > 1) us += 4.0 + 2.0 * s * m * n * 4 / 5.0e6;
+      if (us < least) least = us, best = {tile, s};
+    }
+  }
+  return best;
+}
+
+static bool aligned16(const void *p, int64_t ld, int64_t extent) {
+  return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && extent % 8 == 0;
+}
+
 template <typename T, bool TA, bool TB>
-int gemm(const Gemm<T> &g, hipStream_t stream) {
+int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
   if (g.m == 0 || g.n == 0) return OBB_OK;
+  if constexpr (sizeof(T) == 2) {
+    // (a workgroup's slab must fit a buffer descriptor: 256 rows, or 64 when the contraction is outermost, below 2 GiB)
+    if (aligned16(g.a, g.lda, TA ? g.m : g.k) && aligned16(g.b, g.ldb, TB ? g.n : g.k) && g.lda < (1 << 22) - 256 && g.ldb < (1 << 22) - 256) {
+      const Plan p = plan16(g.m, g.n, g.k);
+      if (int rc = gemm_mfma<T, TA, TB>(g, p.tile, p.splits, ws, stream)) return rc;
+      return p.splits > 1 ? join_splits(g, ws, p.splits, stream) : OBB_OK;
+    }
+  }
   const int64_t tm = (g.m + GT - 1) / GT, tn = (g.n + GT - 1) / GT;
   if (tm * tn > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many tiles (%lld x %lld)", (long long)tm, (long long)tn);
   gemm_general_kernel<T, TA, TB><<<(unsigned)(tm * tn), 256, 0, stream>>>(g, tn);
@@ -151,9 +225,9 @@ static int check_sizes(const char *who, int64_t m, int64_t n, int64_t k, int dty
                                                                                 : [&] { using T = _Float16; return CALL; }())
 
 template <typename T, bool TA, bool TB>
-static int plain_gemm(const void *a, int64_t lda, const void *b, int64_t ldb, int64_t m, int64_t n, int64_t k, void *c, hipStream_t stream) {
+static int plain_gemm(const void *a, int64_t lda, const void *b, int64_t ldb, int64_t m, int64_t n, int64_t k, void *c, void *ws, hipStream_t stream) {
   Gemm<T> g = {(const T *)a, (const T *)b, lda, ldb, m, n, k, nullptr, nullptr, 0, (T *)c, nullptr, OBB_ACT_NONE};
-  return gemm<T, TA, TB>(g, stream);
+  return gemm<T, TA, TB>(g, (float *)ws, stream);
 }
 
 }  // namespace lin
@@ -165,7 +239,11 @@ using namespace obb::lin;
 extern "C" size_t obb_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype, int op) {
   if (m < 0 || n < 0 || k < 0 || bad_dtype(dtype)) return 0;
   if (op == OBB_LINEAR_ACT_BACKWARD) return align_up((size_t)colsum_chunks(m, n) * (size_t)n * 4, 256);
-  return 0;
+  if (op == OBB_LINEAR_BACKWARD_INPUT) std::swap(n, k);            // (m, k) = (m, n) (n, k)
+  if (op == OBB_LINEAR_BACKWARD_WEIGHT) { const int64_t t = m; m = n; n = k; k = t; }   // (n, k) = (n, m) (m, k)
+  if (dtype == OBB_F32) return 0;
+  const Plan p = plan16(m, n, k);
+  return p.splits > 1 ? align_up((size_t)p.splits * (size_t)m * (size_t)n * 4, 256) : 0;
 }
 
 extern "C" int obb_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, const void *res,
@@ -179,7 +257,7 @@ extern "C" int obb_linear_forward(const void *x, int64_t ldx, const void *w, int
   if (ws_bytes < obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_FORWARD)) return set_err(OBB_EWORKSPACE, "obb_linear_forward: workspace too small");
   return OBB_LIN_DISPATCH(dtype, ([&] {
     Gemm<T> g = {(const T *)x, (const T *)w, ldx, ldw, m, n, k, (const T *)bias, (const T *)res, ldr, (T *)y, z, act};
-    return gemm<T, false, false>(g, (hipStream_t)stream);
+    return gemm<T, false, false>(g, (float *)ws, (hipStream_t)stream);
   }()));
 }
 
@@ -205,7 +283,7 @@ extern "C" int obb_linear_backward_input(const void *dz, const void *w, int64_t 
   if (ldw < k) return set_err(OBB_EINVAL, "obb_linear_backward_input: row pitch below the row length");
   if (ws_bytes < obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_BACKWARD_INPUT))
     return set_err(OBB_EWORKSPACE, "obb_linear_backward_input: workspace too small");
-  return OBB_LIN_DISPATCH(dtype, (plain_gemm<T, false, true>(dz, n, w, ldw, m, k, n, dx, (hipStream_t)stream)));
+  return OBB_LIN_DISPATCH(dtype, (plain_gemm<T, false, true>(dz, n, w, ldw, m, k, n, dx, ws, (hipStream_t)stream)));
 }
 
 extern "C" int obb_linear_backward_weight(const void *dz, const void *x, int64_t ldx, int64_t m, int64_t n, int64_t k, int dtype,
@@ -216,5 +294,5 @@ extern "C" int obb_linear_backward_weight(const void *dz, const void *x, int64_t
   if (m > 1 && ldx < k) return set_err(OBB_EINVAL, "obb_linear_backward_weight: row pitch below the row length");
   if (ws_bytes < obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_BACKWARD_WEIGHT))
     return set_err(OBB_EWORKSPACE, "obb_linear_backward_weight: workspace too small");
-  return OBB_LIN_DISPATCH(dtype, (plain_gemm<T, true, true>(dz, n, x, ldx, n, k, m, dw, (hipStream_t)stream)));
+  return OBB_LIN_DISPATCH(dtype, (plain_gemm<T, true, true>(dz, n, x, ldx, n, k, m, dw, ws, (hipStream_t)stream)));
 }

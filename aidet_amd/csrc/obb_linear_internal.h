@@ -66,5 +66,81 @@ __device__ __forceinline__ void epilogue(const Gemm<T> &g, int64_t m, int64_t n,
   g.y[at] = from_f32<T>(act_value(acc, g.act));
 }
 
+// What eight consecutive columns n .. n + 7 need of the epilogue whatever their row: the bias, and whether 16-byte accesses
+// are possible (all eight inside, rows and pointers aligned).
+struct Columns {
+  float bias[8];
+  bool whole, whole_res;
+  template <typename T> __device__ __forceinline__ void load(const Gemm<T> &g, int64_t n) {
+    constexpr uintptr_t A = 15;
+    whole = n + 8 <= g.n && (g.n * sizeof(T) & A) == 0 && ((uintptr_t)g.y & A) == 0 && ((uintptr_t)g.z & A) == 0;
+    whole_res = whole && (g.ldr * sizeof(T) & A) == 0 && ((uintptr_t)g.res & A) == 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) bias[e] = g.bias && n + e < g.n ? to_f32(g.bias[n + e]) : 0.f;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void epilogue8(const Gemm<T> &g, const Columns &c, int64_t m, int64_t n, f32x4 lo, f32x4 hi) {
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  float v[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = (e < 4 ? lo[e] : hi[e - 4]) + c.bias[e];
+  const int64_t at = m * g.n + n;
+  if (c.whole) {
+    if (g.res) {
+      const T *r = g.res + m * g.ldr + n;
+      if (c.whole_res) {
+        const t8 q = *(const t8 *)r;
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += to_f32((T)q[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] += to_f32(r[e]);
+      }
+    }
+    if (g.z) {
+      *(f32x4 *)(g.z + at) = f32x4{v[0], v[1], v[2], v[3]};
+      *(f32x4 *)(g.z + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    }
+    t8 out;
+#pragma unroll
+    for (int e = 0; e < 8; e++) out[e] = from_f32<T>(act_value(v[e], g.act));
+    *(t8 *)(g.y + at) = out;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (n + e < g.n) {
+        float u = v[e];
+        if (g.res) u += to_f32(g.res[m * g.ldr + n + e]);
+        if (g.z) g.z[at + e] = u;
+        g.y[at + e] = from_f32<T>(act_value(u, g.act));
+      }
+  }
+}
+
+// the sums of one split, (m, n) fp32 in the workspace
+__device__ __forceinline__ void store8_partial(float *p, int64_t cols, int64_t m, int64_t n, f32x4 lo, f32x4 hi) {
+  float *at = p + m * cols + n;
+  if (n + 8 <= cols && (cols & 3) == 0) {
+    *(f32x4 *)at = lo;
+    *(f32x4 *)(at + 4) = hi;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (n + e < cols) at[e] = e < 4 ? lo[e] : hi[e - 4];
+  }
+}
+
+// the splits' sums, joined in their order, and the epilogue
+template <typename T> int join_splits(const Gemm<T> &g, const float *partial, int splits, hipStream_t stream);
+
+// How a product is cut: tile edge and number of splits of K.
+struct Plan { int tile, splits; };
+Plan plan16(int64_t m, int64_t n, int64_t k);
+
+// 16-bit operands whose contiguous extents are multiples of 8 and whose rows are 16-byte aligned (obb_linear_mfma.hip)
+template <typename T, bool TA, bool TB> int gemm_mfma(const Gemm<T> &g, int tile, int splits, float *partial, hipStream_t stream);
+
 }  // namespace lin
 }  // namespace obb

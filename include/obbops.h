@@ -725,7 +725,9 @@ OBB_API int obb_topk_distill_backward(const void *logits_dev, int64_t ld, int64_
 #define OBB_TUNE_NMS_RESOLVE_TAIL 19   /* resolve, bit 0: the last <= 4 edges per thread of a shard are retired from registers (1, default) or swept through memory (0); bit 1: the first sweep uses agent-scope loads like the others (measurement only); bit 2: the resolve reports itself stalled (test hook for OBB_ESTALLED) */
 #define OBB_TUNE_NMS_RESOLVE_PARTS 20   /* resolve of calls of >= 2^18 boxes: workgroups per edge shard (1 .. 16; never more than half of what the device keeps resident) */
 #define OBB_TUNE_NMS_RETAIN 21          /* 0: OBB_NMS_RETAIN is ignored (every call runs the frame launch): A/B measurements */
-#define OBB_TUNE_COUNT 22
+#define OBB_TUNE_LINEAR_TILE 22         /* fused linear layer: tile of the 16-bit product */
+#define OBB_TUNE_LINEAR_SPLITS 23       /* fused linear layer: splits of the contraction */
+#define OBB_TUNE_COUNT 24
 OBB_API int obb_set_tuning(int knob, int64_t value);
 /* which route the calling thread's last synchronous obb_nms_*_f32 call took: 0 fused (one workgroup), 1 direct, 2 sorted,
  * 4 grid, 5 grid gave up (crowded cell) and the call was repeated on the sorted route; -1 none yet */
