@@ -112,23 +112,24 @@ int join_splits(const Gemm<T> &g, const float *partial, int splits, hipStream_t 
 
 Plan plan16(int64_t m, int64_t n, int64_t k) {
   const int force = (int)tuning(OBB_TUNE_LINEAR_TILE, 0), force_s = (int)tuning(OBB_TUNE_LINEAR_SPLITS, 0);
-  // the cheapest of the tiles and splits by the time of a slab (64 k) of one workgroup, the rounds the device needs, and what
-  // the splits' sums cost to write and read back
+  // The cheapest by: rounds the device needs x slabs of a workgroup x the time of a slab (by how many workgroups share a CU),
+  // plus the splits' sums written and read back (at 4.7 TB/s) and the launch that joins them.
+  // Measured at 2000 x 12544 x 1024 bf16: 256 / 8 splits 64 us, 128 / 4 69, 128 / 2 81, 64 / 1 85, 128 / 1 137, 256 / 1 229;
+  // at 2000 x 1024 x 1024: 64 / 1 17, 128 / 1 18, with 2 splits 23.
   const int64_t slabs = (k + 63) / 64;
   Plan best = {64, 1};
   double least = 1e30;
   for (int tile : {256, 128, 64}) {
     if (force && tile != force) continue;
-    const double slab_us = tile == 256 ? 1.75 : tile == 128 ? 0.51 : 0.17;      // (of one workgroup, its share of a full device)
-    const int together = tile == 256 ? 1 : tile == 128 ? 2 : 4;
     const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
-    for (int s = 1; s <= 16 && s <= (slabs > 1 ? slabs : 1); s *= 2) {
+    const int fit = tile == 256 ? 1 : tile == 128 ? 2 : 4;
+    for (int s = 1; s <= 16 && (s == 1 || s * 2 <= slabs); s *= 2) {
       if (force_s && s != force_s) continue;
-      const int64_t rounds = (tiles * s + 256 * together - 1) / (256 * together);
-      const int64_t per_cu = (tiles * s + 255) / 256;
-      const double one = slab_us * (per_cu < together ? (per_cu < 1 ? 1 : per_cu) : together);
-      double us = rounds * ((slabs + s - 1) / s) * one + 2.0;
-      if (s > 1) us += 4.0 + 2.0 * s * m * n * 4 / 5.0e6;
+      const int64_t per_cu = (tiles * s + 255) / 256, rounds = (per_cu + fit - 1) / fit;
+      const int share = per_cu < fit ? (int)per_cu : fit;
+      const double slab = tile == 256 ? 1.4 : tile == 128 ? (share == 1 ? 0.66 : 1.0) : (share == 1 ? 0.36 : share == 2 ? 0.43 : 0.75);
+      double us = 3.0 + rounds * (2.0 + slab * ((slabs + s - 1) / s));
+      if (s > 1) us += 4.0 + 2.0 * s * m * n * 4 / 4.7e6;
       if (us < least) least = us, best = {tile, s};
     }
   }

@@ -22,11 +22,27 @@ template <> __device__ __forceinline__ float to_f32<__bf16>(__bf16 v) { return (
 template <> __device__ __forceinline__ float to_f32<_Float16>(_Float16 v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 
-// act(z).  gelu is the exact one, z Phi(z); silu z / (1 + e^-z) (e^-z = inf below -88: z / inf = -0, the limit).
+// erf by Abramowitz and Stegun 7.1.26: |error| <= 1.5e-7, one exp and one reciprocal.  gelu needs erf to an absolute error: it
+// is z / 2 times 1 + erf.
+__device__ __forceinline__ float erf_as(float x) {
+  const float a = fabsf(x), t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, a, 1.f));
+  float p = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  p = __builtin_fmaf(p, t, 1.421413741f);
+  p = __builtin_fmaf(p, t, -0.284496736f);
+  p = __builtin_fmaf(p, t, 0.254829592f);
+  const float e = __builtin_amdgcn_exp2f(a * a * -1.4426950408889634f);
+  return copysignf(__builtin_fmaf(-p * t, e, 1.f), x);
+}
+
+// act(z).  gelu is the exact one, z Phi(z); silu z / (1 + e^-z) (e^-z = inf below -88: z times 0 = -0, the limit).
 __device__ __forceinline__ float act_value(float z, int act) {
   if (act == OBB_ACT_RELU) return z != z ? z : fmaxf(z, 0.f);   // (a NaN stays one)
-  if (act == OBB_ACT_GELU) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-  if (act == OBB_ACT_SILU) return z / (1.f + expf(-z));
+  if (act == OBB_ACT_GELU) {
+    const float h = 0.5f * z;
+    // (-inf: the limit is 0, not the -inf * 0 of the formula)
+    return z < -40.f ? -0.f : __builtin_fmaf(h, erf_as(z * 0.70710678118654752f), h);
+  }
+  if (act == OBB_ACT_SILU) return z < -104.f ? -0.f : z * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
   return z;
 }
 
@@ -57,13 +73,13 @@ struct Gemm {
   int act;
 };
 
-template <typename T>
+template <typename T, int ACT = -1>
 __device__ __forceinline__ void epilogue(const Gemm<T> &g, int64_t m, int64_t n, float acc) {
   if (g.bias) acc += to_f32(g.bias[n]);
   if (g.res) acc += to_f32(g.res[m * g.ldr + n]);
   const int64_t at = m * g.n + n;
   if (g.z) g.z[at] = acc;
-  g.y[at] = from_f32<T>(act_value(acc, g.act));
+  g.y[at] = from_f32<T>(act_value(acc, ACT < 0 ? g.act : ACT));
 }
 
 // What eight consecutive columns n .. n + 7 need of the epilogue whatever their row: the bias, and whether 16-byte accesses
@@ -119,17 +135,31 @@ __device__ __forceinline__ void epilogue8(const Gemm<T> &g, const Columns &c, in
   }
 }
 
-// the sums of one split, (m, n) fp32 in the workspace
-__device__ __forceinline__ void store8_partial(float *p, int64_t cols, int64_t m, int64_t n, f32x4 lo, f32x4 hi) {
-  float *at = p + m * cols + n;
-  if (n + 8 <= cols && (cols & 3) == 0) {
-    *(f32x4 *)at = lo;
-    *(f32x4 *)(at + 4) = hi;
-  } else {
+// four consecutive columns of a row, aligned (the caller has checked), bias added already
+template <typename T, int ACT>
+__device__ __forceinline__ void epilogue4(const Gemm<T> &g, int64_t m, int64_t n, f32x4 v) {
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  if (g.res) {
+    const t4 q = *(const t4 *)(g.res + m * g.ldr + n);
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (n + e < cols) at[e] = e < 4 ? lo[e] : hi[e - 4];
+    for (int e = 0; e < 4; e++) v[e] += to_f32((T)q[e]);
   }
+  const int64_t at = m * g.n + n;
+  if (g.z) *(f32x4 *)(g.z + at) = v;
+  t4 out;
+#pragma unroll
+  for (int e = 0; e < 4; e++) out[e] = from_f32<T>(act_value(v[e], ACT));
+  *(t4 *)(g.y + at) = out;
+}
+
+// the sums of one split, (m, n) fp32 in the workspace; `whole`: rows are multiples of four columns
+__device__ __forceinline__ void store4_partial(float *p, int64_t cols, int64_t m, int64_t n, f32x4 v, bool whole) {
+  float *at = p + m * cols + n;
+  if (whole) *(f32x4 *)at = v;
+  else
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (n + e < cols) at[e] = v[e];
 }
 
 // the splits' sums, joined in their order, and the epilogue

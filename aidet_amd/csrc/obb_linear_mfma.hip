@@ -1,14 +1,17 @@
 // obb_linear_mfma.hip -- the tiled product of 16-bit operands: C (M, N) = sum_k A(m, k) B(n, k), epilogue of the fused
 // linear layer, either operand stored with its contraction innermost ("rows") or outermost ("columns").
 //
-// A workgroup owns a BM x BN tile and walks K in slabs of 64 through two LDS buffers: while one is multiplied, the next
-// slab travels memory -> LDS (buffer loads that write LDS, no registers in between) and one barrier a slab hands over.
+// A workgroup owns a BM x BN tile and walks K in steps of 32 through a ring of five LDS slots: memory -> LDS without registers
+// in between (buffer loads that write LDS), LDS -> fragments one step ahead, fragments -> matrix instructions.  One barrier a
+// step: behind it the slot whose fragments everybody has taken is filled again, four steps before it is needed.
+// What bounds it: the matrix pipe, once the loads' latency is covered.  With two slots of 64 k (one in flight at a time) the
+// loads alone took 815 of 908 us at 8192 x 4096 x 16384; it is their latency, not their bytes (L2 hits 79 %).
 //
-// LDS layout.  "rows": [row][64 k], 128 bytes a row in eight 16-byte chunks, chunk c of row r kept at c ^ (r & 7): the 16
-// rows of a fragment, read 16 bytes a lane, spread over all banks.  "columns": [k][rows], chunk c of slab row k kept at
-// c ^ 2 (k & 3 | k >> 1 & 4), read with the transposing LDS load (a group of 16 lanes reads 4 k x 16 rows and each lane gets
-// 4 k of one row): the eight slab rows that 32 lanes read at once fall on different banks, and pairs of chunks stay together.
-// The loads write LDS in lane order, so the exchange is made in the address that a lane reads from memory.
+// LDS layout.  "rows": two rows of 32 k (64 bytes) make a line of eight 16-byte chunks; chunk c of row r sits at
+// ((r & 1) 4 + c) ^ (r >> 1 & 7) of line r / 2: the 16 rows of a fragment, read 16 bytes a lane, spread over all banks.
+// "columns": [k][rows], chunk c of row k kept at c ^ turn(k), read with the transposing LDS load (a group of 16 lanes reads
+// 4 k x 16 rows and each lane gets 4 k of one row): the eight rows of k that 32 lanes read at once fall on different banks, and
+// pairs of chunks stay together.  The loads write LDS in lane order, so the exchange is made in the address a lane reads.
 //
 // Edges: a lane whose chunk lies outside the operand reads at an offset beyond the buffer descriptor's size, which gives
 // zeros; a chunk never straddles an edge, because the caller has checked that the contiguous extent is a multiple of 8.
@@ -17,7 +20,8 @@
 namespace obb {
 namespace lin {
 
-constexpr int BK = 64;
+constexpr int BK = 64, RING = 5;
+
 
 template <typename T> struct Vec8;
 template <> struct Vec8<__bf16> { typedef bf16x8 v; };
@@ -29,28 +33,34 @@ __device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) { return __built
 typedef __attribute__((address_space(3))) char lds_char;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// 64 lanes x 16 bytes from (descriptor, per-lane offset) to 1 KiB of LDS at `lds`
-__device__ __forceinline__ void load_to_lds(__amdgpu_buffer_rsrc_t rsrc, uint32_t off, uint32_t lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void *)(uintptr_t)lds, 16, (int)off, 0, 0, 0);
+// 64 lanes x 16 bytes from (descriptor, per-lane offset) to 1 KiB of LDS at `lds`.  In assembly, because the compiler would wait
+// for the builtin's loads before every transposing LDS read; it has no register result, and wait_and_meet() waits for it.
+// (m0 needs one wait state before its use, a descriptor register that a vector instruction wrote five: s_nop 4 covers both.)
+__device__ __forceinline__ void load_to_lds(u32x4 rsrc, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(off), "s"(rsrc) : "memory");
 }
-// this wave's loads have landed and its LDS reads are done; then the workgroup meets
-__device__ __forceinline__ void wait_and_meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
+// all but this wave's last `LEFT` loads have landed and its LDS reads are done; then the workgroup meets
+template <int LEFT> __device__ __forceinline__ void wait_and_meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((LEFT & 15) | 0x70 | (LEFT >> 4) << 14);   // vmcnt(LEFT) lgkmcnt(0)
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 constexpr uint32_t OUTSIDE = 0x80000000u;   // beyond every descriptor's size
 
-// the exchange of chunks in row k of a "columns" slab
+// the exchange of chunks in row k of a "columns" slot
 template <int R> __device__ __forceinline__ int turn(int k) { return (2 * ((k & 3) | (k >> 1 & 4))) & (R / 8 - 1); }
 
-// One operand's slab of `R` rows x 64 k: `R` / 8 wave loads, dealt over the workgroup's waves.
+// One operand's slot of `R` rows x 32 k: `R` / 16 wave loads, dealt over the workgroup's waves.
 template <typename T, int R, int WAVES, bool TR>
 struct Slab {
   static constexpr int LOADS = R / 8 / WAVES;
   static constexpr int BYTES = R * BK * 2;
   static_assert(LOADS * 8 * WAVES == R, "");
-  uint32_t off[LOADS];   // byte offset within the slab, or OUTSIDE
+  uint32_t off[LOADS];   // byte offset within the step, or OUTSIDE
   int kof[LOADS];        // first k of the lane's chunk
-  const char *base;      // of the slab at k = 0
-  int64_t step;          // bytes from slab to slab
+  const char *base;      // of step 0
+  int64_t step;          // bytes from step to step
 
   __device__ __forceinline__ void init(const T *p, int64_t ld, int64_t r0, int64_t rows, int64_t k0, int wave, int lane) {
     base = (const char *)p + (TR ? (k0 * ld + r0) * 2 : (r0 * ld + k0) * 2);
@@ -69,60 +79,66 @@ struct Slab {
       }
     }
   }
-  // slab number t (k from t * BK, `rest` of them inside the operand) to LDS
+  // load i of slab t (`rest` of its k inside the operand: none or fewer gives zeros) to the slot at `lds`
+  __device__ __forceinline__ void issue(int i, int64_t t, int64_t rest, uint32_t lds, int wave) const {
+    const int left = rest < BK ? (rest < 0 ? 0 : (int)rest) : BK;
+    const uint64_t at = (uint64_t)(base + t * step);
+    const u32x4 rsrc = {(uint32_t)at, (uint32_t)(at >> 32) & 0xffffu, OUTSIDE - 1, 0x00020000u};
+    load_to_lds(rsrc, kof[i] < left ? off[i] : OUTSIDE, lds + (uint32_t)(wave * LOADS + i) * 1024u);
+  }
   __device__ __forceinline__ void issue(int64_t t, int64_t rest, uint32_t lds, int wave) const {
-    const int left = rest < BK ? (int)rest : BK;
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)(base + t * step), 0, OUTSIDE - 1, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < LOADS; i++)
-      load_to_lds(rsrc, kof[i] < left ? off[i] : OUTSIDE, lds + (uint32_t)(wave * LOADS + i) * 1024u);
+    for (int i = 0; i < LOADS; i++) issue(i, t, rest, lds, wave);
   }
 };
 
-// The 16 rows x 32 k fragment at (row, 32 ks): lane l holds row l & 15, k = 8 (l >> 4) ... + 7.
+// One lane's eight k of one row of a 16 x 32 fragment at (row, 32 h): lane l holds row l % 16, k = 8 (l / 16) ... + 7.
 template <typename T, int R, bool TR>
-__device__ __forceinline__ typename Vec8<T>::v fragment(const char *lds, int row, int ks, int lane) {
+__device__ __forceinline__ typename Vec8<T>::v fragment(const char *lds, int row, int h, int lane) {
   if constexpr (TR) {
-    const int g = lane >> 4, s = lane & 15, k = ks * 32 + 8 * g + (s >> 2), c = (row >> 3) + ((s & 3) >> 1);
-    // (k & 4 never enters the exchange: both halves sit at the same place of their slab rows)
+    const int s = lane & 15, k = 32 * h + 8 * (lane >> 4) + (s >> 2), c = (row >> 3) + ((s & 3) >> 1);
+    // (k & 4 never enters the exchange: both halves sit at the same place of their rows)
     const int at = (k * (R / 8) + (c ^ turn<R>(k))) * 16 + (s & 1) * 8;
     union { s16x4 h[2]; typename Vec8<T>::v v; } u;
     u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds + at));
     u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(lds + at + 4 * (R / 8) * 16));
     return u.v;
   } else {
-    const int r = row + (lane & 15), c = ks * 4 + (lane >> 4);
+    const int r = row + (lane & 15), c = 4 * h + (lane >> 4);
     return *(const typename Vec8<T>::v *)(lds + r * 128 + ((c ^ (r & 7)) << 4));
   }
 }
 
 // Workgroup number -> tile.  Workgroups go to the 8 dies in turn: the number is turned so that a die gets a run of tiles, and
 // the runs walk blocks of 8 tile rows, so that the tiles a die works on at a time share rows of both operands in its L2.
-__device__ __forceinline__ void tile_of(int64_t wg, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn) {
-  const int64_t total = tiles_m * tiles_n, per = total / 8, rest = total % 8, die = wg % 8, i = wg / 8;
-  const int64_t t = die * per + (die < rest ? die : rest) + i;
-  constexpr int64_t G = 8;
-  const int64_t group = t / (G * tiles_n), first = group * G, size = tiles_m - first < G ? tiles_m - first : G;
-  tm = first + (t - group * G * tiles_n) % size;
-  tn = (t - group * G * tiles_n) / size;
+__device__ __forceinline__ void tile_of(uint32_t wg, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm, uint32_t &tn) {
+  const uint32_t total = tiles_m * tiles_n, per = total / 8, rest = total % 8, die = wg % 8, i = wg / 8;
+  const uint32_t t = die * per + (die < rest ? die : rest) + i;
+  constexpr uint32_t G = 8;
+  const uint32_t group = t / (G * tiles_n), first = group * G, size = tiles_m - first < G ? tiles_m - first : G, in = t - first * tiles_n;
+  tn = in / size;
+  tm = first + in - tn * size;
 }
 
 // BM x BN tile on WM x WN waves; split s of `splits` takes slabs [s * per, s * per + per) and, with more than one split, leaves its
 // sums in partial[s].  Operands enter the matrix instruction swapped, so that a lane holds four consecutive n of one m.
-template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB>
-__global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, int64_t tiles_m, int64_t tiles_n, int splits, int64_t per, float *partial) {
+template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB, int ACT>
+__global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, uint32_t tiles_m, uint32_t tiles_n, uint32_t splits, int64_t per, float *partial) {
   constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Slab<T, BM, WAVES, TA> SA;
   typedef Slab<T, BN, WAVES, TB> SB;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * (SA::BYTES + SB::BYTES)];
+  static_assert(BM == BN, "slots serve either operand");
+  constexpr uint32_t SLOT = SA::BYTES;
+  constexpr int LOADS = SA::LOADS + SB::LOADS;
+  __shared__ __attribute__((aligned(1024))) char lds[RING * SLOT];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-  const int split = (int)(blockIdx.x % splits);
-  int64_t tm, tn;
+  const uint32_t split = blockIdx.x % splits;
+  uint32_t tm, tn;
   tile_of(blockIdx.x / splits, tiles_m, tiles_n, tm, tn);
-  const int64_t m0 = tm * BM, n0 = tn * BN, k0 = (int64_t)split * per * BK;
-  const int64_t kk = g.k - k0 < per * BK ? g.k - k0 : per * BK;      // this split's k
-  const int64_t slabs = (kk + BK - 1) / BK;
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN, k0 = (int64_t)split * per * BK;
+  const int64_t kk = g.k - k0 < per * BK ? g.k - k0 : per * BK;      // this split's k (none: its sums are zeros)
+  const int64_t slabs = kk > 0 ? (kk + BK - 1) / BK : 0;
 
   SA sa;
   SB sb;
@@ -130,75 +146,118 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, int64
   sb.init(g.b, g.ldb, n0, g.n, k0, wave, lane);
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_char *)lds;
   f32x4 acc[FM][FN] = {};
+  typename Vec8<T>::v fa[2][FM], fb[2][FN];
+  // fragment f (B's first) of half h
+  auto read = [&](int f, int h, uint32_t at_a, uint32_t at_b) {
+    if (f < FN) fb[h][f] = fragment<T, BN, TB>(lds + at_b, wn + 16 * f, h, lane);
+    else fa[h][f - FN] = fragment<T, BM, TA>(lds + at_a, wm + 16 * (f - FN), h, lane);
+  };
+  // Half a slab: half h is multiplied while the other half's fragments are read from (at_a, at_b) and one operand's slab t goes
+  // out to slot `to`.  Loads and reads are dealt evenly between the matrix instructions, and the compiler is held to that order:
+  // a wave issues in order, and loads in a row would hold back its matrix instructions while the address unit (16 cycles
+  // a load, all waves') is busy.
+  auto half = [&](int h, uint32_t at_a, uint32_t at_b, const auto &s, int64_t t, uint32_t to) {
+    constexpr int Q = SA::LOADS, R = (FM + FN + Q - 1) / Q;
+#pragma unroll
+    for (int q = 0; q < Q; q++) {
+#pragma unroll
+      for (int f = q * R; f < q * R + R && f < FM + FN; f++) read(f, h ^ 1, at_a, at_b);
+      s.issue(q, t, kk - t * BK, lds0 + to, wave);
+#pragma unroll
+      for (int i = q * FM / Q; i < (q + 1) * FM / Q; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[h][j], fa[h][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Slots in turn: A 0, B 0, A 1, B 1, A 2, then B 2 where A 0 was, ...  (past the last slab every lane is outside and the
+  // loads give zeros: no branch in the loop)
   if (slabs > 0) {
+    auto after = [](uint32_t at) { return at + SLOT == RING * SLOT ? 0 : at + SLOT; };
     sa.issue(0, kk, lds0, wave);
-    sb.issue(0, kk, lds0 + SA::BYTES, wave);
-    wait_and_meet();
-  }
-  for (int64_t t = 0; t < slabs; t++) {
-    const uint32_t here = (t & 1) * (SA::BYTES + SB::BYTES);
-    if (t + 1 < slabs) {
-      const uint32_t next = lds0 + (SA::BYTES + SB::BYTES - here);
-      sa.issue(t + 1, kk - (t + 1) * BK, next, wave);
-      sb.issue(t + 1, kk - (t + 1) * BK, next + SA::BYTES, wave);
+    sb.issue(0, kk, lds0 + SLOT, wave);
+    sa.issue(1, kk - BK, lds0 + 2 * SLOT, wave);
+    sb.issue(1, kk - BK, lds0 + 3 * SLOT, wave);
+    wait_and_meet<SA::LOADS + SB::LOADS>();
+    uint32_t at_a = 0, at_b = SLOT, free_slot = 4 * SLOT;
+#pragma unroll
+    for (int f = 0; f < FM + FN; f++) read(f, 0, at_a, at_b);
+    for (int64_t t = 0; t < slabs; t++) {
+      half(0, at_a, at_b, sa, t + 2, free_slot);   // (where B t - 1 was)
+      wait_and_meet<SA::LOADS>();                  // A, B t + 1 have landed, everybody has slab t's fragments
+      const uint32_t to = at_a;
+      free_slot = at_b;
+      at_a = after(at_b), at_b = after(at_a);
+      half(1, at_a, at_b, sb, t + 2, to);
     }
-    const char *pa = lds + here, *pb = lds + here + SA::BYTES;
-#pragma unroll
-    for (int ks = 0; ks < BK / 32; ks++) {
-      typename Vec8<T>::v fa[FM], fb[FN];
-#pragma unroll
-      for (int j = 0; j < FN; j++) fb[j] = fragment<T, BN, TB>(pb, wn + 16 * j, ks, lane);
-#pragma unroll
-      for (int i = 0; i < FM; i++) fa[i] = fragment<T, BM, TA>(pa, wm + 16 * i, ks, lane);
-#pragma unroll
-      for (int i = 0; i < FM; i++)
-#pragma unroll
-        for (int j = 0; j < FN; j++) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
-    }
-    wait_and_meet();
   }
-  // Out through LDS, a wave on its own part of it: the sums are laid down as rows of C columns (16-byte chunk c of row r at
-  // c ^ r: the 16 rows that are written at once, and the rows read at once, fall on different banks) and leave as runs of
-  // whole rows, eight columns a lane.
-  constexpr int C = FN * 16, ROWS = sizeof(lds) / (WAVES * C * 4) < FM * 16 ? sizeof(lds) / (WAVES * C * 4) : FM * 16;
-  constexpr int CH = C / 4, LPR = C / 8, RPP = 64 / LPR;
-  char *mine = lds + wave * ROWS * C * 4;
-  const int64_t n = n0 + wn + (lane % LPR) * 8;
-  float *part = splits > 1 ? partial + (int64_t)split * g.m * g.n : nullptr;
-  Columns cols;
-  cols.load(g, n);
+  wait_and_meet<0>();
+  const int64_t nw = n0 + wn + 4 * (lane >> 4);      // of the lane's four columns in fragment j: + 16 j
+  if (splits > 1) {
+    float *part = partial + (int64_t)split * g.m * g.n;
+    const bool whole = (g.n & 3) == 0;
 #pragma unroll
-  for (int i0 = 0; i0 < FM; i0 += ROWS / 16) {
+    for (int i = 0; i < FM; i++) {
+      const int64_t m = m0 + wm + 16 * i + (lane & 15);
 #pragma unroll
-    for (int i = i0; i < i0 + ROWS / 16; i++)
+      for (int j = 0; j < FN; j++)
+        if (m < g.m && nw + 16 * j < g.n) store4_partial(part, g.n, m, nw + 16 * j, acc[i][j], whole);
+    }
+    return;
+  }
+  const bool whole = (g.n & 3) == 0 && ((uintptr_t)g.y & 7) == 0 && ((uintptr_t)g.res & 7) == 0 && (g.ldr & 3) == 0;
+  if (whole) {
+    // four columns of a row as one access: the fragments of a row's 64 columns leave one after the other and L2 joins them
+    f32x4 bias[FN] = {};
+    if (g.bias)
 #pragma unroll
-      for (int j = 0; j < FN; j++) {
-        const int r = (i - i0) * 16 + (lane & 15), c = j * 4 + (lane >> 4);
-        *(f32x4 *)(mine + r * C * 4 + ((c ^ (r & (CH - 1))) << 4)) = acc[i][j];
-      }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      for (int j = 0; j < FN; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (nw + 16 * j < g.n) bias[j][e] = to_f32(g.bias[nw + 16 * j + e]);
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+      const int64_t m = m0 + wm + 16 * i + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < FN; j++)
+        if (m < g.m && nw + 16 * j < g.n) epilogue4<T, ACT>(g, m, nw + 16 * j, acc[i][j] + bias[j]);
+    }
+  } else {
+    // element by element, in a loop, from LDS: a wave lays down 16 rows at a time
+    float *mine = (float *)lds + wave * 16 * FN * 16;
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+#pragma unroll
+      for (int j = 0; j < FN; j++) *(f32x4 *)(mine + (lane & 15) * FN * 16 + 16 * j + 4 * (lane >> 4)) = acc[i][j];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 1
-    for (int p = 0; p < ROWS; p += RPP) {
-      const int r = p + lane / LPR, c = (lane % LPR) * 2;
-      const int64_t m = m0 + wm + i0 * 16 + r;
-      const f32x4 lo = *(const f32x4 *)(mine + r * C * 4 + ((c ^ (r & (CH - 1))) << 4));
-      const f32x4 hi = *(const f32x4 *)(mine + r * C * 4 + (((c + 1) ^ (r & (CH - 1))) << 4));
-      if (m < g.m && n < g.n) {
-        if (part) store8_partial(part, g.n, m, n, lo, hi);
-        else epilogue8(g, cols, m, n, lo, hi);
+      for (int e = lane; e < 16 * FN * 16; e += 64) {
+        const int64_t m = m0 + wm + 16 * i + e / (FN * 16), n = n0 + wn + e % (FN * 16);
+        if (m < g.m && n < g.n) epilogue<T, ACT>(g, m, n, mine[e]);
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB, int ACT>
+static int launch_act(const Gemm<T> &g, uint32_t tm, uint32_t tn, uint32_t splits, int64_t per, float *partial, hipStream_t stream) {
+  gemm_mfma_kernel<T, BM, BN, WM, WN, TA, TB, ACT><<<tm * tn * splits, WM * WN * 64, 0, stream>>>(g, tm, tn, splits, per, partial);
+  OBB_LAUNCH_CHECK();
+  return OBB_OK;
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB>
 static int launch(const Gemm<T> &g, int splits, float *partial, hipStream_t stream) {
   const int64_t tm = (g.m + BM - 1) / BM, tn = (g.n + BN - 1) / BN, slabs = (g.k + BK - 1) / BK, per = (slabs + splits - 1) / splits;
   if (tm * tn * splits > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many tiles (%lld x %lld)", (long long)tm, (long long)tn);
-  gemm_mfma_kernel<T, BM, BN, WM, WN, TA, TB><<<(unsigned)(tm * tn * splits), WM * WN * 64, 0, stream>>>(g, tm, tn, splits, per, partial);
-  OBB_LAUNCH_CHECK();
-  return OBB_OK;
+  const int act = splits > 1 ? OBB_ACT_NONE : g.act;
+  if constexpr (!TA && !TB) {                        // (the gradients' products have no activation)
+    if (act == OBB_ACT_RELU) return launch_act<T, BM, BN, WM, WN, TA, TB, OBB_ACT_RELU>(g, (uint32_t)tm, (uint32_t)tn, splits, per, partial, stream);
+    if (act == OBB_ACT_GELU) return launch_act<T, BM, BN, WM, WN, TA, TB, OBB_ACT_GELU>(g, (uint32_t)tm, (uint32_t)tn, splits, per, partial, stream);
+    if (act == OBB_ACT_SILU) return launch_act<T, BM, BN, WM, WN, TA, TB, OBB_ACT_SILU>(g, (uint32_t)tm, (uint32_t)tn, splits, per, partial, stream);
+  }
+  return launch_act<T, BM, BN, WM, WN, TA, TB, OBB_ACT_NONE>(g, (uint32_t)tm, (uint32_t)tn, splits, per, partial, stream);
 }
 
 template <typename T, bool TA, bool TB>
