@@ -162,12 +162,79 @@ __device__ __forceinline__ void store4_partial(float *p, int64_t cols, int64_t m
       if (n + e < cols) at[e] = v[e];
 }
 
+// Workgroup number -> tile.  Workgroups go to the 8 dies in turn: the number is turned so that a die gets a run of tiles, and
+// the runs walk blocks of 8 tile rows, so that the tiles a die works on at a time share rows of both operands in its L2.
+__device__ __forceinline__ void tile_of(uint32_t wg, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm, uint32_t &tn) {
+  const uint32_t total = tiles_m * tiles_n, per = total / 8, rest = total % 8, die = wg % 8, i = wg / 8;
+  const uint32_t t = die * per + (die < rest ? die : rest) + i;
+  constexpr uint32_t G = 8;
+  const uint32_t group = t / (G * tiles_n), first = group * G, size = tiles_m - first < G ? tiles_m - first : G, in = t - first * tiles_n;
+  tn = in / size;
+  tm = first + in - tn * size;
+}
+
+// A wave's FM x FN fragments of sums go out.  They are C transposed: lane l holds, of fragment (i, j), row m0 + 16 i + l % 16
+// and the four columns n0 + 16 j + 4 (l / 16) ... + 3.  `part`: the split's sums instead of the epilogue; `mine`: 256 FN
+// floats of LDS of the wave's own (used where rows are not aligned).
+template <typename T, int ACT, int FM, int FN>
+__device__ __forceinline__ void tile_out(const Gemm<T> &g, const f32x4 (&acc)[FM][FN], int64_t m0, int64_t n0, float *part, float *mine, int lane) {
+  const int64_t nw = n0 + 4 * (lane >> 4);      // of the lane's four columns in fragment j: + 16 j
+  if (part) {
+    const bool whole = (g.n & 3) == 0;
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+      const int64_t m = m0 + 16 * i + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < FN; j++)
+        if (m < g.m && nw + 16 * j < g.n) store4_partial(part, g.n, m, nw + 16 * j, acc[i][j], whole);
+    }
+    return;
+  }
+  constexpr uintptr_t A = 4 * sizeof(T) - 1;
+  const bool whole = (g.n & 3) == 0 && ((uintptr_t)g.y & A) == 0 && ((uintptr_t)g.res & A) == 0 && (g.ldr & 3) == 0;
+  if (whole) {
+    // four columns of a row as one access: the fragments of a row's 64 columns leave one after the other and L2 joins them
+    f32x4 bias[FN] = {};
+    if (g.bias)
+#pragma unroll
+      for (int j = 0; j < FN; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (nw + 16 * j < g.n) bias[j][e] = to_f32(g.bias[nw + 16 * j + e]);
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+      const int64_t m = m0 + 16 * i + (lane & 15);
+#pragma unroll
+      for (int j = 0; j < FN; j++)
+        if (m < g.m && nw + 16 * j < g.n) epilogue4<T, ACT>(g, m, nw + 16 * j, acc[i][j] + bias[j]);
+    }
+  } else {
+    // element by element, in a loop, from LDS: a wave lays down 16 rows at a time
+#pragma unroll
+    for (int i = 0; i < FM; i++) {
+#pragma unroll
+      for (int j = 0; j < FN; j++) *(f32x4 *)(mine + (lane & 15) * FN * 16 + 16 * j + 4 * (lane >> 4)) = acc[i][j];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+      for (int e = lane; e < 16 * FN * 16; e += 64) {
+        const int64_t m = m0 + 16 * i + e / (FN * 16), n = n0 + e % (FN * 16);
+        if (m < g.m && n < g.n) epilogue<T, ACT>(g, m, n, mine[e]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+}
+
 // the splits' sums, joined in their order, and the epilogue
 template <typename T> int join_splits(const Gemm<T> &g, const float *partial, int splits, hipStream_t stream);
 
 // How a product is cut: tile edge and number of splits of K.
 struct Plan { int tile, splits; };
 Plan plan16(int64_t m, int64_t n, int64_t k);
+Plan plan32(int64_t m, int64_t n, int64_t k);
+
+// fp32 operands, any alignment (obb_linear_split.hip)
+template <bool TA, bool TB> int gemm_split(const Gemm<float> &g, int tile, int splits, float *partial, hipStream_t stream);
 
 // 16-bit operands whose contiguous extents are multiples of 8 and whose rows are 16-byte aligned (obb_linear_mfma.hip)
 template <typename T, bool TA, bool TB> int gemm_mfma(const Gemm<T> &g, int tile, int splits, float *partial, hipStream_t stream);

@@ -109,17 +109,6 @@ __device__ __forceinline__ typename Vec8<T>::v fragment(const char *lds, int row
   }
 }
 
-// Workgroup number -> tile.  Workgroups go to the 8 dies in turn: the number is turned so that a die gets a run of tiles, and
-// the runs walk blocks of 8 tile rows, so that the tiles a die works on at a time share rows of both operands in its L2.
-__device__ __forceinline__ void tile_of(uint32_t wg, uint32_t tiles_m, uint32_t tiles_n, uint32_t &tm, uint32_t &tn) {
-  const uint32_t total = tiles_m * tiles_n, per = total / 8, rest = total % 8, die = wg % 8, i = wg / 8;
-  const uint32_t t = die * per + (die < rest ? die : rest) + i;
-  constexpr uint32_t G = 8;
-  const uint32_t group = t / (G * tiles_n), first = group * G, size = tiles_m - first < G ? tiles_m - first : G, in = t - first * tiles_n;
-  tn = in / size;
-  tm = first + in - tn * size;
-}
-
 // BM x BN tile on WM x WN waves; split s of `splits` takes slabs [s * per, s * per + per) and, with more than one split, leaves its
 // sums in partial[s].  Operands enter the matrix instruction swapped, so that a lane holds four consecutive n of one m.
 template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB, int ACT>
@@ -192,52 +181,7 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, uint3
     }
   }
   wait_and_meet<0>();
-  const int64_t nw = n0 + wn + 4 * (lane >> 4);      // of the lane's four columns in fragment j: + 16 j
-  if (splits > 1) {
-    float *part = partial + (int64_t)split * g.m * g.n;
-    const bool whole = (g.n & 3) == 0;
-#pragma unroll
-    for (int i = 0; i < FM; i++) {
-      const int64_t m = m0 + wm + 16 * i + (lane & 15);
-#pragma unroll
-      for (int j = 0; j < FN; j++)
-        if (m < g.m && nw + 16 * j < g.n) store4_partial(part, g.n, m, nw + 16 * j, acc[i][j], whole);
-    }
-    return;
-  }
-  const bool whole = (g.n & 3) == 0 && ((uintptr_t)g.y & 7) == 0 && ((uintptr_t)g.res & 7) == 0 && (g.ldr & 3) == 0;
-  if (whole) {
-    // four columns of a row as one access: the fragments of a row's 64 columns leave one after the other and L2 joins them
-    f32x4 bias[FN] = {};
-    if (g.bias)
-#pragma unroll
-      for (int j = 0; j < FN; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (nw + 16 * j < g.n) bias[j][e] = to_f32(g.bias[nw + 16 * j + e]);
-#pragma unroll
-    for (int i = 0; i < FM; i++) {
-      const int64_t m = m0 + wm + 16 * i + (lane & 15);
-#pragma unroll
-      for (int j = 0; j < FN; j++)
-        if (m < g.m && nw + 16 * j < g.n) epilogue4<T, ACT>(g, m, nw + 16 * j, acc[i][j] + bias[j]);
-    }
-  } else {
-    // element by element, in a loop, from LDS: a wave lays down 16 rows at a time
-    float *mine = (float *)lds + wave * 16 * FN * 16;
-#pragma unroll
-    for (int i = 0; i < FM; i++) {
-#pragma unroll
-      for (int j = 0; j < FN; j++) *(f32x4 *)(mine + (lane & 15) * FN * 16 + 16 * j + 4 * (lane >> 4)) = acc[i][j];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-      for (int e = lane; e < 16 * FN * 16; e += 64) {
-        const int64_t m = m0 + wm + 16 * i + e / (FN * 16), n = n0 + wn + e % (FN * 16);
-        if (m < g.m && n < g.n) epilogue<T, ACT>(g, m, n, mine[e]);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-  }
+  tile_out<T, ACT, FM, FN>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * g.n : nullptr, (float *)lds + wave * 256 * FN, lane);
 }
 
 template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB, int ACT>
