@@ -203,7 +203,9 @@ def lib():
         L.obb_linear_backward_input.restype = i32
         L.obb_linear_backward_weight.argtypes = [vp, vp, i64, i64, i64, i64, i32, vp, vp, sz, vp]
         L.obb_linear_backward_weight.restype = i32
-        L.obb_topk_distill_forward.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, i32, i32, f32, vp, vp, vp, f32, vp, vp]
+        L.obb_topk_distill_forward.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, i32, i32, f32, vp, vp, vp, f32, vp, vp, sz, vp]
+        L.obb_topk_distill_workspace_bytes.argtypes = [i64, i64]
+        L.obb_topk_distill_workspace_bytes.restype = sz
         L.obb_topk_distill_forward.restype = i32
         L.obb_topk_distill_backward.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, i32, i32, f32, vp, vp, vp, i64, f32, vp, i64, vp]
         L.obb_topk_distill_backward.restype = i32

@@ -35,19 +35,63 @@ struct Args {
   int64_t ldd;
 };
 
-// max and sum of exp(x - max) of a set; the empty set is {-inf, 0}.  -inf adds nothing; NaN and +inf end as a NaN sum.
+// max and sum of exp((x - max) / T) of a set; the empty set is {-inf, 0}.  -inf adds nothing; NaN and +inf end as a NaN sum.
 struct Stat { float m, s; };
-__device__ __forceinline__ void stat_add(Stat &a, float x, float c2) {
-  if (x > a.m) {
-    a.s = a.s * exp2f((a.m - x) * c2) + 1.f;
-    a.m = x;
-  } else if (x != -INFINITY) {
-    a.s += exp2f((x - a.m) * c2);
+template <int N> __device__ __forceinline__ void stat_add(Stat &a, const float (&x)[N], float c2) {
+  float top = x[0];
+#pragma unroll
+  for (int i = 1; i < N; i++) top = fmaxf(top, x[i]);           // (NaN only if all are)
+  if (top > a.m) {
+    a.s *= __builtin_amdgcn_exp2f((a.m - top) * c2);
+    a.m = top;
   }
+  const float base = a.m == -INFINITY ? 0.f : a.m;              // (nothing but -inf so far: they add exp(-inf) = 0, a NaN itself)
+#pragma unroll
+  for (int i = 0; i < N; i++) a.s += __builtin_amdgcn_exp2f((x[i] - base) * c2);
 }
 __device__ __forceinline__ Stat stat_join(Stat a, Stat b, float c2) {
   const float m = fmaxf(a.m, b.m);
-  return {m, (a.m == m ? a.s : a.s * exp2f((a.m - m) * c2)) + (b.m == m ? b.s : b.s * exp2f((b.m - m) * c2))};
+  return {m, (a.m == m ? a.s : a.s * __builtin_amdgcn_exp2f((a.m - m) * c2)) + (b.m == m ? b.s : b.s * __builtin_amdgcn_exp2f((b.m - m) * c2))};
+}
+
+// A run of n elements at any alignment by NT threads: 16-byte loads, `U` of them in flight; f(element number, values[]) gets
+// whole 16-byte groups, or single elements at the ends.
+template <typename T, int NT, int U, typename F>
+__device__ __forceinline__ void sweep(const T *p, int64_t n, int tid, F f) {
+  constexpr int W = 16 / sizeof(T);
+  typedef T tw __attribute__((ext_vector_type(W)));
+  const int64_t off = ((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T), head = off < n ? off : n;
+  const int64_t groups = (n - head) / W;
+  if (tid < head) {
+    const float x[1] = {(float)p[tid]};
+    f((int64_t)tid, x);
+  }
+  const tw *q = (const tw *)(p + head);
+  int64_t g = tid;
+  for (; g + (U - 1) * NT < groups; g += U * NT) {
+    tw v[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) v[u] = q[g + u * NT];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      float x[W];
+#pragma unroll
+      for (int i = 0; i < W; i++) x[i] = (float)v[u][i];
+      f(head + (g + u * NT) * W, x);
+    }
+  }
+  for (; g < groups; g += NT) {
+    const tw v = q[g];
+    float x[W];
+#pragma unroll
+    for (int i = 0; i < W; i++) x[i] = (float)v[i];
+    f(head + g * W, x);
+  }
+  const int64_t tail = head + groups * W + tid;
+  if (tail < n) {
+    const float x[1] = {(float)p[tail]};
+    f(tail, x);
+  }
 }
 
 __device__ __forceinline__ float value_at(const Args &a, int64_t at) {
@@ -85,6 +129,34 @@ __device__ __forceinline__ float2 stage_entries(const Args &a, int64_t row, int 
   return make_float2(m, s);
 }
 
+// sum of p_j (log p_j - log q_j) over this thread's entries, from the row's {max, sum} and the teacher's
+template <typename T, int NT>
+__device__ __forceinline__ float entries_loss(const Args &a, const T *s, Stat st, float2 t, const int *idx, const float *val, int tid, float c2) {
+  float l = 0.f;
+  const float log_sum = logf(st.s), log_tsum = logf(t.y), inv = 1.f / t.y;
+  for (int j = tid; j < a.k; j += NT)
+    if (idx[j] >= 0 && val[j] != -INFINITY) {
+      const float p = __builtin_amdgcn_exp2f((val[j] - t.x) * c2) * inv;
+      if (p != 0.f) l += p * (((val[j] - t.x) * a.inv_temp - log_tsum) - (((float)s[idx[j]] - st.m) * a.inv_temp - log_sum));
+    }
+  return l;
+}
+
+// ---- long rows: a workgroup per row or per part of one ------------------------------------------------------------------
+// Bound by reading the logits: 16-byte loads, four in flight a thread.  With fewer rows than would fill the device a row is cut
+// into parts, whose {max, sum} a second launch joins.
+__device__ __forceinline__ Stat block_stat(Stat st, float *red, float c2) {
+  const float m = block_reduce(st.m, red, [](float x, float y) { return fmaxf(x, y); });
+  const float s = block_reduce(st.m == m ? st.s : st.s * __builtin_amdgcn_exp2f((st.m - m) * c2), red, [](float x, float y) { return x + y; });
+  return {m, s};
+}
+
+__device__ __forceinline__ void finish_row(const Args &a, int64_t row, Stat st, float2 t, float l) {
+  const float w = a.weight ? a.weight[row] : 1.f;
+  a.loss[row] = w == 0.f || t.x == -INFINITY ? 0.f : l * (a.temp * a.temp * w);
+  if (a.stats) a.stats[row] = make_float2(st.m, st.s);
+}
+
 template <typename T>
 __global__ __launch_bounds__(256) void distill_forward_kernel(Args a) {
   __shared__ int idx[KMAX];
@@ -93,53 +165,211 @@ __global__ __launch_bounds__(256) void distill_forward_kernel(Args a) {
   const float c2 = a.inv_temp * LOG2E;
   const T *s = (const T *)a.logits + row * a.ld;
   Stat st = {-INFINITY, 0.f};
-  for (int64_t v = threadIdx.x; v < a.classes; v += 256) stat_add(st, (float)s[v], c2);
-  const float m = block_reduce(st.m, red, [](float x, float y) { return fmaxf(x, y); });
-  const float sum = block_reduce(st.m == m ? st.s : st.s * exp2f((st.m - m) * c2), red, [](float x, float y) { return x + y; });
+  sweep<T, 256, 4>(s, a.classes, threadIdx.x, [&](int64_t, const auto &x) { stat_add(st, x, c2); });
+  st = block_stat(st, red, c2);
   const float2 t = stage_entries(a, row, idx, val, red, c2);
-  const float w = a.weight ? a.weight[row] : 1.f;
-  float l = 0.f;
-  const float log_sum = logf(sum), log_tsum = logf(t.y), inv = 1.f / t.y;
-  for (int j = threadIdx.x; j < a.k; j += 256)
-    if (idx[j] >= 0 && val[j] != -INFINITY) {
-      const float p = exp2f((val[j] - t.x) * c2) * inv;
-      if (p != 0.f) l += p * (((val[j] - t.x) * a.inv_temp - log_tsum) - (((float)s[idx[j]] - m) * a.inv_temp - log_sum));
-    }
-  l = block_reduce(l, red, [](float x, float y) { return x + y; });
-  if (threadIdx.x == 0) {
-    a.loss[row] = w == 0.f || t.x == -INFINITY ? 0.f : l * (a.temp * a.temp * w);
-    if (a.stats) a.stats[row] = make_float2(m, sum);
-  }
+  const float l = block_reduce(entries_loss<T, 256>(a, s, st, t, idx, val, threadIdx.x, c2), red, [](float x, float y) { return x + y; });
+  if (threadIdx.x == 0) finish_row(a, row, st, t, l);
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void distill_backward_kernel(Args a) {
+__global__ __launch_bounds__(256) void distill_part_kernel(Args a, int64_t per, float2 *part) {
+  __shared__ float red[4];
+  const int64_t row = blockIdx.y, v0 = blockIdx.x * per, n = a.classes - v0 < per ? a.classes - v0 : per;
+  const float c2 = a.inv_temp * LOG2E;
+  Stat st = {-INFINITY, 0.f};
+  sweep<T, 256, 4>((const T *)a.logits + row * a.ld + v0, n, threadIdx.x, [&](int64_t, const auto &x) { stat_add(st, x, c2); });
+  st = block_stat(st, red, c2);
+  if (threadIdx.x == 0) part[row * gridDim.x + blockIdx.x] = make_float2(st.m, st.s);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void distill_join_kernel(Args a, const float2 *part, int parts) {
   __shared__ int idx[KMAX];
   __shared__ float val[KMAX], red[4];
   const int64_t row = blockIdx.x;
   const float c2 = a.inv_temp * LOG2E;
-  const T *s = (const T *)a.logits + row * a.ld;
-  T *d = (T *)a.dlogits + row * a.ldd;
+  Stat st = {-INFINITY, 0.f};
+  for (int i = threadIdx.x; i < parts; i += 256) {
+    const float2 p = part[row * parts + i];
+    st = stat_join(st, Stat{p.x, p.y}, c2);
+  }
+  st = block_stat(st, red, c2);
+  const float2 t = stage_entries(a, row, idx, val, red, c2);
+  const float l = block_reduce(entries_loss<T, 256>(a, (const T *)a.logits + row * a.ld, st, t, idx, val, threadIdx.x, c2), red,
+                               [](float x, float y) { return x + y; });
+  if (threadIdx.x == 0) finish_row(a, row, st, t, l);
+}
+
+// One pass: g (q - 0) everywhere, then the entries' classes of this part once more with their p.  Rows go from the last to the
+// first: what the forward pass read last may still be in the cache in front of the memory.
+template <typename T>
+__global__ __launch_bounds__(256) void distill_backward_kernel(Args a, int64_t per) {
+  constexpr int W = 16 / sizeof(T), SLOTS = 2 * KMAX;
+  typedef T tw __attribute__((ext_vector_type(W)));
+  __shared__ int idx[KMAX], seen[SLOTS], twice;
+  __shared__ float val[KMAX], red[4];
+  const int64_t row = gridDim.y - 1 - blockIdx.y, v0 = blockIdx.x * per, n = a.classes - v0 < per ? a.classes - v0 : per;
+  const float c2 = a.inv_temp * LOG2E;
+  const T *s = (const T *)a.logits + row * a.ld + v0;
+  T *d = (T *)a.dlogits + row * a.ldd + v0;
   const float w = a.weight ? a.weight[row] : 1.f;
   const float2 st = a.stats[row], t = stage_entries(a, row, idx, val, red, c2);
+  const bool same = (((uintptr_t)s ^ (uintptr_t)d) & 15) == 0;    // 16-byte groups of both fall together
   if (w == 0.f || t.x == -INFINITY) {
-    for (int64_t v = threadIdx.x; v < a.classes; v += 256) d[v] = (T)0.f;
+    for (int64_t v = threadIdx.x; v < n; v += 256) d[v] = (T)0.f;
     return;
   }
   const float g = a.grad[row * a.grad_stride] * a.scale * w * a.temp, inv = 1.f / st.y, tinv = 1.f / t.y;
-  for (int64_t v = threadIdx.x; v < a.classes; v += 256) d[v] = (T)(g * (exp2f(((float)s[v] - st.x) * c2) * inv));
-  __syncthreads();   // (the entries' classes are written again below, by other threads)
+  sweep<T, 256, 4>(s, n, threadIdx.x, [&](int64_t at, const auto &x) {
+    constexpr int N = sizeof(x) / sizeof(float);
+    T out[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) out[i] = (T)(g * (__builtin_amdgcn_exp2f((x[i] - st.x) * c2) * inv));
+    if constexpr (N > 1)
+      if (same) {
+        tw v;
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] = out[i];
+        *(tw *)(d + at) = v;
+        return;
+      }
+#pragma unroll
+    for (int i = 0; i < N; i++) d[at + i] = out[i];
+  });
+  // is an index there twice?  (a table of the indices seen, open addressing: at most half full)
+  if (threadIdx.x == 0) twice = 0;
+  for (int i = threadIdx.x; i < SLOTS; i += 256) seen[i] = -1;
+  __syncthreads();                                    // (the stores above are done before the entries' below)
   for (int j = threadIdx.x; j < a.k; j += 256) {
     const int i = idx[j];
     if (i < 0) continue;
-    float p = 0.f;   // an index may come twice: the first place writes for all of them
+    for (uint32_t h = (uint32_t)i * 2654435761u >> 21;; h = (h + 1) & (SLOTS - 1)) {
+      const int was = atomicCAS(&seen[h], -1, i);
+      if (was == i) twice = 1;
+      if (was == -1 || was == i) break;
+    }
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < a.k; j += 256) {
+    const int i = idx[j];
+    if (i < v0 || i >= v0 + n) continue;
+    float p = val[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((val[j] - t.x) * c2) * tinv;
     bool first = true;
-    for (int o = 0; o < a.k; o++)
-      if (idx[o] == i) {
-        first = first && o >= j;
-        if (val[o] != -INFINITY) p += exp2f((val[o] - t.x) * c2) * tinv;
+    if (twice) {                                      // the first place writes for all of them
+      p = 0.f;
+      for (int o = 0; o < a.k; o++)
+        if (idx[o] == i) {
+          first = first && o >= j;
+          if (val[o] != -INFINITY) p += __builtin_amdgcn_exp2f((val[o] - t.x) * c2) * tinv;
+        }
+    }
+    if (first) d[i - v0] = (T)(g * (__builtin_amdgcn_exp2f(((float)s[i - v0] - st.x) * c2) * inv - p));
+  }
+}
+
+// ---- short rows: G lanes of a wave per row, its classes in their registers (E = up to 1024 / G each), entries by broadcast ----------
+template <int G, typename F> __device__ __forceinline__ float lanes_reduce(float v, F f) {
+#pragma unroll
+  for (int o = G / 2; o; o >>= 1) v = f(v, __shfl_xor(v, o));
+  return v;
+}
+
+// Entry j = lane + G e of the row: index (-1 = absent) and value; returns {max, sum} of the entries present.
+template <int G>
+__device__ __forceinline__ float2 lane_entries(const Args &a, int64_t row, int lane, float c2, bool live) {
+  float m = -INFINITY, s = 0.f;
+  for (int j = lane; j < a.k; j += G) {
+    const int64_t i = live ? index_at(a, row * a.k + j) : -1;
+    if (i >= 0 && i < a.classes) {
+      const float v = value_at(a, row * a.k + j);
+      m = v > m || v != v ? v : m;
+    }
+  }
+  m = lanes_reduce<G>(m, [](float x, float y) { return x != x ? x : (y != y ? y : fmaxf(x, y)); });
+  for (int j = lane; j < a.k; j += G) {
+    const int64_t i = live ? index_at(a, row * a.k + j) : -1;
+    if (i >= 0 && i < a.classes) {
+      const float v = value_at(a, row * a.k + j);
+      if (v != -INFINITY) s += __builtin_amdgcn_exp2f((v - m) * c2);
+    }
+  }
+  return make_float2(m, lanes_reduce<G>(s, [](float x, float y) { return x + y; }));
+}
+
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void distill_forward_short_kernel(Args a) {
+  const int lane = threadIdx.x % G;
+  const int64_t mine = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  const bool live = mine < a.rows;
+  const int64_t row = live ? mine : a.rows - 1;        // (no lane leaves: the reductions are of whole waves)
+  const float c2 = a.inv_temp * LOG2E;
+  const T *s = (const T *)a.logits + row * a.ld;
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) x[e] = lane + e * G < a.classes ? (float)s[lane + e * G] : -INFINITY;
+  Stat st = {-INFINITY, 0.f};
+  stat_add(st, x, c2);
+  const float m = lanes_reduce<G>(st.m, [](float u, float v) { return fmaxf(u, v); });
+  st.s = lanes_reduce<G>(st.m == m ? st.s : st.s * __builtin_amdgcn_exp2f((st.m - m) * c2), [](float u, float v) { return u + v; });
+  st.m = m;
+  const float2 t = lane_entries<G>(a, row, lane, c2, live);
+  float l = 0.f;
+  const float log_sum = logf(st.s), log_tsum = logf(t.y), inv = 1.f / t.y;
+  for (int j = lane; j < a.k; j += G) {
+    const int64_t i = index_at(a, row * a.k + j);
+    if (i < 0 || i >= a.classes) continue;
+    const float v = value_at(a, row * a.k + j);
+    const float p = v == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((v - t.x) * c2) * inv;
+    if (p != 0.f) l += p * (((v - t.x) * a.inv_temp - log_tsum) - (((float)s[i] - st.m) * a.inv_temp - log_sum));
+  }
+  l = lanes_reduce<G>(l, [](float u, float v) { return u + v; });
+  if (live && lane == 0) finish_row(a, row, st, t, l);
+}
+
+// The entries' p are summed into a row of LDS, one entry after the other (their order is the order of the sum).
+template <typename T, int G, int E>
+__global__ __launch_bounds__(256) void distill_backward_short_kernel(Args a) {
+  __shared__ float probs[256 / G][G * E];
+  const int lane = threadIdx.x % G, sub = threadIdx.x / G;
+  const int64_t mine = (int64_t)blockIdx.x * (256 / G) + sub;
+  const bool live = mine < a.rows;
+  const int64_t row = live ? mine : a.rows - 1;
+  const float c2 = a.inv_temp * LOG2E;
+  const T *s = (const T *)a.logits + row * a.ld;
+  T *d = (T *)a.dlogits + row * a.ldd;
+  float x[E];
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    x[e] = lane + e * G < a.classes ? (float)s[lane + e * G] : -INFINITY;
+    probs[sub][lane + e * G] = 0.f;
+  }
+  const float2 st = a.stats[row], t = lane_entries<G>(a, row, lane, c2, live);
+  const float w = a.weight ? a.weight[row] : 1.f;
+  const bool none = w == 0.f || t.x == -INFINITY;
+  const float g = a.grad[row * a.grad_stride] * a.scale * w * a.temp, inv = 1.f / st.y, tinv = 1.f / t.y;
+  for (int j0 = 0; j0 < a.k; j0 += G) {
+    const int j = j0 + lane;
+    int i = -1;
+    float p = 0.f;
+    if (j < a.k && live) {
+      const int64_t at = index_at(a, row * a.k + j);
+      if (at >= 0 && at < a.classes) {
+        const float v = value_at(a, row * a.k + j);
+        i = (int)at;
+        p = v == -INFINITY ? 0.f : __builtin_amdgcn_exp2f((v - t.x) * c2) * tinv;
       }
-    if (first) d[i] = (T)(g * (exp2f(((float)s[i] - st.x) * c2) * inv - p));
+    }
+    for (int o = 0; o < G && j0 + o < a.k; o++) {
+      const int io = __shfl(i, o, G);
+      const float po = __shfl(p, o, G);
+      if (io >= 0 && io % G == lane) probs[sub][io] += po;     // (a class belongs to one lane: no race)
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < E; e++) {
+    const int v = lane + e * G;
+    if (live && v < a.classes) d[v] = none ? (T)0.f : (T)(g * (__builtin_amdgcn_exp2f((x[e] - st.x) * c2) * inv - probs[sub][v]));
   }
 }
 
@@ -156,6 +386,69 @@ __global__ __launch_bounds__(1024) void distill_sum_kernel(const float *loss, in
     for (int i = 0; i < 16; i++) s += red[i];
     *out = (float)(s * (double)scale);
   }
+}
+
+// A row is cut into parts where rows alone would not give the device two workgroups a CU; a part is worth 4096 classes at least.
+static int parts_of(int64_t rows, int64_t classes) {
+  const int64_t want = rows > 0 ? (512 + rows - 1) / rows : 1, have = classes / 4096;
+  return (int)(want < have ? want : (have < 1 ? 1 : have));
+}
+
+// rows of up to 1024 classes: lanes of a wave
+template <typename T, bool FORWARD> static bool short_rows(const Args &a, hipStream_t st) {
+#define OBB_SHORT(G, E)                                                                                               \
+  if (a.classes <= G * E) {                                                                                           \
+    const unsigned blocks = (unsigned)((a.rows + 256 / G - 1) / (256 / G));                                           \
+    if (FORWARD) distill_forward_short_kernel<T, G, E><<<blocks, 256, 0, st>>>(a);                                    \
+    else distill_backward_short_kernel<T, G, E><<<blocks, 256, 0, st>>>(a);                                           \
+    return true;                                                                                                      \
+  }
+  OBB_SHORT(16, 1)
+  OBB_SHORT(16, 4)
+  OBB_SHORT(64, 4)
+  OBB_SHORT(64, 16)
+#undef OBB_SHORT
+  return false;
+}
+
+template <typename T> static int forward(const Args &a, float2 *ws, hipStream_t st) {
+  if (!short_rows<T, true>(a, st)) {
+    const int parts = parts_of(a.rows, a.classes);
+    if (parts == 1) distill_forward_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a);
+    else {
+      const int64_t per = ((a.classes + parts - 1) / parts + 7) / 8 * 8;
+      distill_part_kernel<T><<<dim3(parts, (unsigned)a.rows), 256, 0, st>>>(a, per, ws);
+      OBB_LAUNCH_CHECK();
+      distill_join_kernel<T><<<(unsigned)a.rows, 256, 0, st>>>(a, ws, parts);
+    }
+  }
+  OBB_LAUNCH_CHECK();
+  return OBB_OK;
+}
+
+template <typename T> static int backward(Args a, hipStream_t st) {
+  if (!short_rows<T, false>(a, st)) {
+    const int parts = parts_of(a.rows, a.classes);
+    const int64_t per = parts == 1 ? a.classes : ((a.classes + parts - 1) / parts + 7) / 8 * 8;
+    // (a grid's second dimension ends at 65535: more rows go in several launches, the last rows first)
+    for (int64_t end = a.rows; end > 0;) {
+      const int64_t n = end < 65535 ? end : 65535, r0 = end - n;
+      Args b = a;
+      b.rows = n;
+      b.logits = (const T *)a.logits + r0 * a.ld;
+      b.dlogits = (T *)a.dlogits + r0 * a.ldd;
+      b.values = (const char *)a.values + r0 * a.k * (a.vtype == OBB_F32 ? 4 : 2);
+      b.indices = (const char *)a.indices + r0 * a.k * (a.wide_index ? 8 : 4);
+      b.weight = a.weight ? a.weight + r0 : nullptr;
+      b.stats = a.stats + r0;
+      b.grad = a.grad + r0 * a.grad_stride;
+      distill_backward_kernel<T><<<dim3(parts, (unsigned)n), 256, 0, st>>>(b, per);
+      OBB_LAUNCH_CHECK();
+      end = r0;
+    }
+  }
+  OBB_LAUNCH_CHECK();
+  return OBB_OK;
 }
 
 static int check(const char *who, int64_t rows, int64_t classes, int64_t ld, int dtype, int k, int vtype, int itype, float temperature) {
@@ -175,23 +468,29 @@ static int check(const char *who, int64_t rows, int64_t classes, int64_t ld, int
 using namespace obb;
 using namespace obb::dst;
 
+extern "C" size_t obb_topk_distill_workspace_bytes(int64_t rows, int64_t classes) {
+  if (rows <= 0 || classes <= 1024) return 0;
+  const int parts = parts_of(rows, classes);
+  return parts > 1 ? align_up((size_t)rows * parts * sizeof(float2), 256) : 0;
+}
+
 extern "C" int obb_topk_distill_forward(const void *logits, int64_t ld, int64_t rows, int64_t classes, int dtype,
                                         const void *values, const void *indices, int k, int vtype, int index_bytes,
                                         float temperature, const float *weight, float *row_loss, float *stats, float scale,
-                                        float *loss, void *stream) {
+                                        float *loss, void *ws, size_t ws_bytes, void *stream) {
   if (int rc = check("obb_topk_distill_forward", rows, classes, ld, dtype, k, vtype, index_bytes, temperature)) return rc;
   if (rows > 0 && (!row_loss || (classes > 0 && !logits) || (k > 0 && (!values || !indices))))
     return set_err(OBB_EINVAL, "obb_topk_distill_forward: null pointer");
+  if (ws_bytes < obb_topk_distill_workspace_bytes(rows, classes) || (!ws && ws_bytes))
+    return set_err(OBB_EWORKSPACE, "obb_topk_distill_forward: workspace too small");
   hipStream_t st = (hipStream_t)stream;
   Args a = {};
   a.logits = logits; a.ld = ld; a.rows = rows; a.classes = classes; a.values = values; a.indices = indices;
   a.k = k; a.vtype = vtype; a.wide_index = index_bytes == 8; a.inv_temp = 1.f / temperature; a.temp = temperature;
   a.weight = weight; a.loss = row_loss; a.stats = (float2 *)stats;
   if (rows > 0) {
-    if (dtype == OBB_F32) distill_forward_kernel<float><<<(unsigned)rows, 256, 0, st>>>(a);
-    else if (dtype == OBB_BF16) distill_forward_kernel<__bf16><<<(unsigned)rows, 256, 0, st>>>(a);
-    else distill_forward_kernel<_Float16><<<(unsigned)rows, 256, 0, st>>>(a);
-    OBB_LAUNCH_CHECK();
+    const int rc = dtype == OBB_F32 ? forward<float>(a, (float2 *)ws, st) : dtype == OBB_BF16 ? forward<__bf16>(a, (float2 *)ws, st) : forward<_Float16>(a, (float2 *)ws, st);
+    if (rc) return rc;
   }
   if (loss) {
     distill_sum_kernel<<<1, 1024, 0, st>>>(row_loss, rows, scale, loss);
@@ -216,9 +515,5 @@ extern "C" int obb_topk_distill_backward(const void *logits, int64_t ld, int64_t
   a.k = k; a.vtype = vtype; a.wide_index = index_bytes == 8; a.inv_temp = 1.f / temperature; a.temp = temperature;
   a.weight = weight; a.stats = (float2 *)stats; a.grad = grad; a.grad_stride = grad_stride; a.scale = scale;
   a.dlogits = dlogits; a.ldd = ldd;
-  if (dtype == OBB_F32) distill_backward_kernel<float><<<(unsigned)rows, 256, 0, st>>>(a);
-  else if (dtype == OBB_BF16) distill_backward_kernel<__bf16><<<(unsigned)rows, 256, 0, st>>>(a);
-  else distill_backward_kernel<_Float16><<<(unsigned)rows, 256, 0, st>>>(a);
-  OBB_LAUNCH_CHECK();
-  return OBB_OK;
+  return dtype == OBB_F32 ? backward<float>(a, st) : dtype == OBB_BF16 ? backward<__bf16>(a, st) : backward<_Float16>(a, st);
 }

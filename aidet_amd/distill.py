@@ -41,10 +41,12 @@ class TopkDistillFunction(Function):
             stats = torch.empty((rows, 2), dtype=torch.float32, device=dev) if logits.requires_grad else None
             total = None if scale is None else torch.empty((), dtype=torch.float32, device=dev)
             if rows > 0 or total is not None:
+                nbytes = _lib.lib().obb_topk_distill_workspace_bytes(rows, classes)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
                 _lib.check(_lib.lib().obb_topk_distill_forward(
                     s.data_ptr(), ld, rows, classes, _lib.DTYPES[s.dtype], v.data_ptr(), i.data_ptr(), k, _lib.DTYPES[v.dtype],
                     i.element_size(), temperature, _ptr(w), row_loss.data_ptr(), _ptr(stats), 1. if scale is None else scale,
-                    _ptr(total), _lib.stream_ptr(dev)))
+                    _ptr(total), _ptr(ws), nbytes, _lib.stream_ptr(dev)))
         ctx.args = (temperature, scale)
         ctx.save_for_backward(logits, v, i, w, stats)
         return row_loss if scale is None else total

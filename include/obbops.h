@@ -682,15 +682,17 @@ OBB_API int obb_linear_backward_weight(const void *dz_dev, const void *x_dev, in
  *   weight_dev        (rows) fp32, or NULL = 1;   k <= OBB_DISTILL_MAX_K
  *   row_loss_dev      (rows) fp32;   stats_dev (rows, 2) fp32, what the backward needs (NULL: no backward follows)
  *   loss_dev          one fp32, or NULL: only the rows' losses are wanted
+ *   workspace_dev     obb_topk_distill_workspace_bytes(rows, classes) bytes (16-byte aligned; 0 bytes: may be NULL)
  *   grad_dev          grad_stride 0: one fp32 (of loss; `scale` as in the forward), 1: (rows) fp32 (of row_loss; scale 1)
  * Replaces: nothing of the reference (its heads train on hard labels); stands beside rbbox_target
  *           (mmdet/core/rbbox/rbbox_target.py:8-93), whose label_weights are its `weight`.
  * ------------------------------------------------------------------------- */
 #define OBB_DISTILL_MAX_K 1024
+OBB_API size_t obb_topk_distill_workspace_bytes(int64_t rows, int64_t classes);
 OBB_API int obb_topk_distill_forward(const void *logits_dev, int64_t ld, int64_t rows, int64_t classes, int dtype,
                                      const void *values_dev, const void *indices_dev, int k, int vtype, int index_bytes,
                                      float temperature, const float *weight_dev, float *row_loss_dev, float *stats_dev,
-                                     float scale, float *loss_dev, void *stream);
+                                     float scale, float *loss_dev, void *workspace_dev, size_t workspace_bytes, void *stream);
 OBB_API int obb_topk_distill_backward(const void *logits_dev, int64_t ld, int64_t rows, int64_t classes, int dtype,
                                       const void *values_dev, const void *indices_dev, int k, int vtype, int index_bytes,
                                       float temperature, const float *weight_dev, const float *stats_dev,

@@ -124,7 +124,7 @@ def test_c_abi_refusals_without_gpu():
     one, null = ctypes.c_void_p(256), None     # (never dereferenced: validation fails first)
 
     def fwd(rows=3, classes=4, ld=4, dtype=0, k=2, vtype=0, ib=8, temp=1., s=one, row_loss=one):
-        return L.obb_topk_distill_forward(s, ld, rows, classes, dtype, one, one, k, vtype, ib, temp, null, row_loss, null, 1., null, null)
+        return L.obb_topk_distill_forward(s, ld, rows, classes, dtype, one, one, k, vtype, ib, temp, null, row_loss, null, 1., null, null, 0, null)
     for bad in (dict(rows=-1), dict(classes=-1), dict(k=1025), dict(dtype=3), dict(vtype=-1), dict(ib=2), dict(temp=0.),
                 dict(temp=float('nan')), dict(temp=float('inf')), dict(ld=3), dict(s=null), dict(row_loss=null), dict(rows=1 << 31)):
         assert fwd(**bad) == _lib.OBB_EINVAL, bad
@@ -208,6 +208,27 @@ def test_masked_logits_and_masked_teacher(rows, classes, k):
         logits[0] = -float('inf')                          # no class left: NaN, as log_softmax, in this row alone
         loss = topk_distill_loss(logits, values, indices, reduction='none')
         assert bool(loss[0].isnan()) and bool(loss[1:].isfinite().all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('rows, classes, k', [(7, 13, 5), (5, 200, 9), (4, 1021, 9), (4, 3001, 9), (2, 66001, 20)])
+def test_nan_stays_in_its_row(rows, classes, k):
+    """a NaN logit -- also where every other one is -inf -- makes its row NaN and no other"""
+    from aidet_amd import topk_distill_loss
+    for dtype in TYPES:
+        logits, values, indices = make(rows, classes, k, dtype, seed=12)
+        want = topk_distill_loss(logits, values, indices, reduction='none')
+        for fill in (None, -float('inf')):
+            for at in (0, classes // 2, classes - 1):
+                x = logits.clone()
+                if fill is not None:
+                    x[1] = fill
+                x[1, at] = float('nan')
+                x.requires_grad_(True)
+                got = topk_distill_loss(x, values, indices, reduction='none')
+                assert bool(got[1].isnan()) and torch.equal(got[[0] + list(range(2, rows))], want[[0] + list(range(2, rows))])
+                grad, = torch.autograd.grad(got, x, torch.ones_like(got))
+                assert bool(grad[1].isnan().all()) and bool(grad[0].isfinite().all())
 
 
 @pytest.mark.gpu
