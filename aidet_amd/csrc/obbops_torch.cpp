@@ -246,6 +246,8 @@ at::Tensor rbox_to_poly(const at::Tensor &rboxes) {
 
 }  // namespace
 
+void bind_training_ops(py::module_ &m);   // obbops_torch_train.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "ATen binding of libobbops (rotated IoU / NMS / RoI-Align on gfx950)";
   m.def("version", []() { return obb_version(); });
@@ -273,4 +275,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("channels"), py::arg("height"), py::arg("width"), py::arg("spatial_scale"),
         py::arg("sample_num") = 0, py::arg("aligned") = false);
   m.def("thetaobb2pointobb", &rbox_to_poly, py::arg("rboxes"));
+  bind_training_ops(m);
 }

@@ -4,9 +4,9 @@ The reference imports its compiled ops as sibling modules of the Python wrappers
 (``from . import nms_cpu, nms_cuda``, mmdet/ops/nms/nms_wrapper.py:4;
 ``from . import roi_align_cuda``, mmdet/ops/roi_align/roi_align.py:6).  This is the
 same kind of module for the rotated ops: ``ext().rnms(dets, thr)`` etc. take and return
-``torch.Tensor`` (signatures in aidet_amd/csrc/obbops_torch.cpp).  It is optional: the
-``ctypes`` path of ``aidet_amd._lib`` serves every wrapper of this package; build this
-one with ``aidet_amd.torch_ext.build()`` -- ``torch.utils.cpp_extension.load`` with the
+``torch.Tensor`` (signatures in aidet_amd/csrc/obbops_torch.cpp).  The ``ctypes`` path of
+``aidet_amd._lib`` serves the box and RoI wrappers of this package without it; the differentiable training operators
+(``fused_linear``, ``topk_distill_loss``: aidet_amd/csrc/obbops_torch_train.cpp) need it.  Build it with ``aidet_amd.torch_ext.build()`` -- ``torch.utils.cpp_extension.load`` with the
 extension's build directory in-tree (``__graft_entry__.build()`` and ``setup.py build_ext`` do).
 """
 import importlib.util
@@ -32,14 +32,14 @@ def build(verbose=False):
     lib_dir = os.path.join(here, 'lib')
     if not os.path.exists(os.path.join(lib_dir, 'libobbops.so')):
         raise _lib.ObbOpsError('build libobbops.so first (make -C aidet_amd/csrc)')
-    src = os.path.join(here, 'csrc', 'obbops_torch.cpp')
+    srcs = [os.path.join(here, 'csrc', f) for f in ('obbops_torch.cpp', 'obbops_torch_train.cpp')]
     out = path()
-    if os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(
-            os.path.join(here, '..', 'include', 'obbops.h'))):
+    if os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(f) for f in srcs + [
+            os.path.join(here, '..', 'include', 'obbops.h')]):
         return out
     _lib.lib()   # libobbops.so is loaded before the freshly built module is imported
     cpp_extension.load(
-        name='obbops_torch', sources=[src], build_directory=lib_dir, verbose=verbose, is_python_module=True,
+        name='obbops_torch', sources=srcs, build_directory=lib_dir, verbose=verbose, is_python_module=True,
         extra_include_paths=[os.path.join(here, '..', 'include'), '/opt/rocm/include'],
         extra_cflags=['-O2', '-D__HIP_PLATFORM_AMD__', '-DUSE_ROCM'],
         extra_ldflags=['-L' + lib_dir, '-lobbops', "-Wl,-rpath,'$$ORIGIN'", '-ltorch_hip', '-lc10_hip'],   # ($$: ninja escape)
