@@ -167,6 +167,12 @@ int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
       if (int rc = gemm_mfma<T, TA, TB>(g, p.tile, p.splits, ws, stream)) return rc;
       return p.splits > 1 ? join_splits(g, ws, p.splits, stream) : OBB_OK;
     }
+    if (tuning(OBB_TUNE_LINEAR_TILE, 0) != 1) {
+      // (the same splits: the workspace is sized without looking at pointers)
+      const Plan p = plan16(g.m, g.n, g.k);
+      if (int rc = gemm_ragged<T, TA, TB>(g, p.tile, p.splits, ws, stream)) return rc;
+      return p.splits > 1 ? join_splits(g, ws, p.splits, stream) : OBB_OK;
+    }
   }
   if constexpr (sizeof(T) == 4) {
     if (tuning(OBB_TUNE_LINEAR_TILE, 0) != 1) {

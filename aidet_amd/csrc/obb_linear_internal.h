@@ -237,6 +237,7 @@ Plan plan32(int64_t m, int64_t n, int64_t k);
 template <bool TA, bool TB> int gemm_split(const Gemm<float> &g, int tile, int splits, float *partial, hipStream_t stream);
 
 // 16-bit operands whose contiguous extents are multiples of 8 and whose rows are 16-byte aligned (obb_linear_mfma.hip)
+template <typename T, bool TA, bool TB> int gemm_ragged(const Gemm<T> &g, int tile, int splits, float *partial, hipStream_t stream);   // any alignment
 template <typename T, bool TA, bool TB> int gemm_mfma(const Gemm<T> &g, int tile, int splits, float *partial, hipStream_t stream);
 
 }  // namespace lin

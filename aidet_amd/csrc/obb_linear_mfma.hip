@@ -184,6 +184,140 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, uint3
   tile_out<T, ACT, FM, FN>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * g.n : nullptr, (float *)lds + wave * 256 * FN, lane);
 }
 
+// ---- the same product where rows or edges are not aligned: through registers ----------------------------------------------
+// 16-byte loads at any element's address (they cost an access more where they cross a line), elements one by one where a
+// chunk crosses the operand's edge, zeros beyond; then into the same LDS layout.  Two LDS slots, one slab ahead in registers.
+template <typename T, int R, bool TR>
+struct Ragged {
+  static constexpr int N = R / 32;                        // chunks a thread (256 threads): R rows x 8 chunks
+  typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
+  u32x4 x[N];
+  const T *base;
+  int64_t ld, rows;
+
+  __device__ __forceinline__ void init(const T *p, int64_t pitch, int64_t r0, int64_t all, int64_t k0) {
+    base = p + (TR ? k0 * pitch + r0 : r0 * pitch + k0);
+    ld = pitch;
+    rows = all - r0 < R ? all - r0 : R;
+  }
+  // eight elements of which `have` exist
+  __device__ __forceinline__ u32x4 chunk(const T *q, int have) const {
+    if (have >= 8) return *(const u32x4u *)q;
+    union { uint16_t h[8]; u32x4 v; } u;
+#pragma unroll
+    for (int e = 0; e < 8; e++) u.h[e] = e < have ? *(const uint16_t *)(q + e) : (uint16_t)0;
+    return u.v;
+  }
+  // slab t, `rest` of its k inside the operand
+  __device__ __forceinline__ void load(int64_t t, int64_t rest) {
+    const int left = rest < BK ? (int)rest : BK;
+    if (left == BK && rows == R) {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const int id = i * 256 + (int)threadIdx.x;
+        const T *q = TR ? base + (t * BK + id / (R / 8)) * ld + id % (R / 8) * 8 : base + (int64_t)(id / 8) * ld + t * BK + id % 8 * 8;
+        x[i] = *(const u32x4u *)q;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const int id = i * 256 + (int)threadIdx.x;
+        const int k = TR ? id / (R / 8) : id % 8 * 8, r = TR ? id % (R / 8) * 8 : id / 8;
+        const int have = TR ? (k < left ? (int)rows - r : 0) : (r < rows ? left - k : 0);
+        x[i] = chunk(TR ? base + (t * BK + k) * ld + r : base + (int64_t)r * ld + t * BK + k, have);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char *lds) const {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const int id = i * 256 + (int)threadIdx.x;
+      if constexpr (TR) {
+        const int k = id / (R / 8), c = id % (R / 8);
+        *(u32x4 *)(lds + (k * (R / 8) + (c ^ turn<R>(k))) * 16) = x[i];
+      } else {
+        const int r = id / 8, c = id % 8;
+        *(u32x4 *)(lds + r * 128 + ((c ^ (r & 7)) << 4)) = x[i];
+      }
+    }
+  }
+};
+
+template <typename T, int B, bool TA, bool TB, int ACT>
+__global__ __launch_bounds__(256) void gemm_ragged_kernel(Gemm<T> g, uint32_t tiles_m, uint32_t tiles_n, uint32_t splits, int64_t per, float *partial) {
+  constexpr int F = B / 32, BYTES = B * BK * 2;            // 2 x 2 waves
+  __shared__ __attribute__((aligned(1024))) char lds[4 * BYTES];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave / 2 * (B / 2), wn = wave % 2 * (B / 2);
+  const uint32_t split = blockIdx.x % splits;
+  uint32_t tm, tn;
+  tile_of(blockIdx.x / splits, tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * B, n0 = (int64_t)tn * B, k0 = (int64_t)split * per * BK;
+  const int64_t kk = g.k - k0 < per * BK ? g.k - k0 : per * BK;
+  const int64_t slabs = kk > 0 ? (kk + BK - 1) / BK : 0;
+  Ragged<T, B, TA> sa;
+  Ragged<T, B, TB> sb;
+  sa.init(g.a, g.lda, m0, g.m, k0);
+  sb.init(g.b, g.ldb, n0, g.n, k0);
+  f32x4 acc[F][F] = {};
+  if (slabs > 0) {
+    sa.load(0, kk);
+    sb.load(0, kk);
+    sa.store(lds);
+    sb.store(lds + BYTES);
+    __syncthreads();
+  }
+#pragma unroll 1
+  for (int64_t t = 0; t < slabs; t++) {
+    char *here = lds + (t & 1) * 2 * BYTES, *next = lds + (~t & 1) * 2 * BYTES;
+    if (t + 1 < slabs) {
+      sa.load(t + 1, kk - (t + 1) * BK);
+      sb.load(t + 1, kk - (t + 1) * BK);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      typename Vec8<T>::v fa[F], fb[F];
+#pragma unroll
+      for (int i = 0; i < F; i++) {
+        fa[i] = fragment<T, B, TA>(here, wm + 16 * i, h, lane);
+        fb[i] = fragment<T, B, TB>(here + BYTES, wn + 16 * i, h, lane);
+      }
+#pragma unroll
+      for (int i = 0; i < F; i++)
+#pragma unroll
+        for (int j = 0; j < F; j++) acc[i][j] = mma(fb[j], fa[i], acc[i][j]);
+    }
+    if (t + 1 < slabs) {                                   // (everybody left that slot at the last barrier)
+      sa.store(next);
+      sb.store(next + BYTES);
+    }
+    __syncthreads();
+  }
+  tile_out<T, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * g.n : nullptr, (float *)lds + wave * 256 * F, lane);
+}
+
+template <typename T, int B, bool TA, bool TB>
+static int launch_ragged(const Gemm<T> &g, int splits, float *partial, hipStream_t stream) {
+  const int64_t tm = (g.m + B - 1) / B, tn = (g.n + B - 1) / B, slabs = (g.k + BK - 1) / BK, per = (slabs + splits - 1) / splits;
+  if (tm * tn * splits > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many tiles (%lld x %lld)", (long long)tm, (long long)tn);
+  const uint32_t grid = (uint32_t)(tm * tn * splits), um = (uint32_t)tm, un = (uint32_t)tn, us = (uint32_t)splits;
+  const int act = splits > 1 ? OBB_ACT_NONE : g.act;
+  if constexpr (!TA && !TB) {
+    if (act == OBB_ACT_RELU) gemm_ragged_kernel<T, B, TA, TB, OBB_ACT_RELU><<<grid, 256, 0, stream>>>(g, um, un, us, per, partial);
+    if (act == OBB_ACT_GELU) gemm_ragged_kernel<T, B, TA, TB, OBB_ACT_GELU><<<grid, 256, 0, stream>>>(g, um, un, us, per, partial);
+    if (act == OBB_ACT_SILU) gemm_ragged_kernel<T, B, TA, TB, OBB_ACT_SILU><<<grid, 256, 0, stream>>>(g, um, un, us, per, partial);
+  }
+  if (act == OBB_ACT_NONE) gemm_ragged_kernel<T, B, TA, TB, OBB_ACT_NONE><<<grid, 256, 0, stream>>>(g, um, un, us, per, partial);
+  OBB_LAUNCH_CHECK();
+  return OBB_OK;
+}
+
+template <typename T, bool TA, bool TB>
+int gemm_ragged(const Gemm<T> &g, int tile, int splits, float *partial, hipStream_t stream) {
+  if (tile == 64) return launch_ragged<T, 64, TA, TB>(g, splits, partial, stream);
+  return launch_ragged<T, 128, TA, TB>(g, splits, partial, stream);
+}
+
 template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB, int ACT>
 static int launch_act(const Gemm<T> &g, uint32_t tm, uint32_t tn, uint32_t splits, int64_t per, float *partial, hipStream_t stream) {
   gemm_mfma_kernel<T, BM, BN, WM, WN, TA, TB, ACT><<<tm * tn * splits, WM * WN * 64, 0, stream>>>(g, tm, tn, splits, per, partial);
@@ -212,6 +346,9 @@ int gemm_mfma(const Gemm<T> &g, int tile, int splits, float *partial, hipStream_
 }
 
 #define INSTANCE(T)                                                                        \
+  template int gemm_ragged<T, false, false>(const Gemm<T> &, int, int, float *, hipStream_t); \
+  template int gemm_ragged<T, false, true>(const Gemm<T> &, int, int, float *, hipStream_t);  \
+  template int gemm_ragged<T, true, true>(const Gemm<T> &, int, int, float *, hipStream_t);   \
   template int gemm_mfma<T, false, false>(const Gemm<T> &, int, int, float *, hipStream_t); \
   template int gemm_mfma<T, false, true>(const Gemm<T> &, int, int, float *, hipStream_t);  \
   template int gemm_mfma<T, true, true>(const Gemm<T> &, int, int, float *, hipStream_t);
