@@ -8,95 +8,31 @@
 namespace obb {
 namespace lin {
 
-// ---- general kernel: any size, any pitch, either operand stored with its contraction outermost ------------------------
-// A workgroup of four waves owns a 64 x 64 tile and walks K in steps of 32: both operands' slabs go element by element
-// (zeros outside) into LDS as [row][k], a wave multiplies its 32 x 32 quarter with 16 x 16 matrix instructions.  The
-// operands enter swapped (B's rows as the instruction's rows), so that a lane ends with four consecutive n of one m.
-constexpr int GT = 64, GK = 32;
-
-template <typename T> struct GeneralPitch { static constexpr int v = GK + 8; };   // 80 B: 16-byte aligned rows
-template <> struct GeneralPitch<float> { static constexpr int v = GK + 4; };
-
-template <typename T, bool TR>
-__device__ __forceinline__ void general_stage(T *lds, const T *p, int64_t ld, int64_t r0, int64_t rows, int64_t k0, int64_t kk) {
-  constexpr int P = GeneralPitch<T>::v;
-  for (int e = threadIdx.x; e < GT * GK; e += 256) {
-    const int r = TR ? e % GT : e / GK, c = TR ? e / GT : e % GK;
-    const int64_t row = r0 + r, k = k0 + c;
-    T v = (T)0.f;
-    if (row < rows && k < kk) v = TR ? p[k * ld + row] : p[row * ld + k];
-    lds[r * P + c] = v;
-  }
-}
-
-__device__ __forceinline__ f32x4 general_mma(const float *b, const float *a, f32x4 c) {
-  constexpr int P = GeneralPitch<float>::v;
-  const int l = threadIdx.x & 63, r = (l & 15) * P, k = l >> 4;
-#pragma unroll
-  for (int s = 0; s < GK; s += 4) c = __builtin_amdgcn_mfma_f32_16x16x4f32(b[r + s + k], a[r + s + k], c, 0, 0, 0);
-  return c;
-}
-__device__ __forceinline__ f32x4 general_mma(const __bf16 *b, const __bf16 *a, f32x4 c) {
-  constexpr int P = GeneralPitch<__bf16>::v;
-  const int l = threadIdx.x & 63, o = (l & 15) * P + (l >> 4) * 8;
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(*(const bf16x8 *)(b + o), *(const bf16x8 *)(a + o), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 general_mma(const _Float16 *b, const _Float16 *a, f32x4 c) {
-  constexpr int P = GeneralPitch<_Float16>::v;
-  const int l = threadIdx.x & 63, o = (l & 15) * P + (l >> 4) * 8;
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const f16x8 *)(b + o), *(const f16x8 *)(a + o), c, 0, 0, 0);
-}
-
-template <typename T, bool TA, bool TB>
-__global__ __launch_bounds__(256) void gemm_general_kernel(Gemm<T> g, int64_t tiles_n) {
-  constexpr int P = GeneralPitch<T>::v;
-  __shared__ __attribute__((aligned(16))) T la[GT * P], lb[GT * P];
-  const int64_t m0 = (int64_t)blockIdx.x / tiles_n * GT, n0 = (int64_t)blockIdx.x % tiles_n * GT;
-  const int w = threadIdx.x >> 6, l = threadIdx.x & 63, wm = (w >> 1) * 32, wn = (w & 1) * 32;
-  f32x4 acc[2][2] = {};
-  for (int64_t k0 = 0; k0 < g.k; k0 += GK) {
-    general_stage<T, TA>(la, g.a, g.lda, m0, g.m, k0, g.k);
-    general_stage<T, TB>(lb, g.b, g.ldb, n0, g.n, k0, g.k);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 2; i++)
-#pragma unroll
-      for (int j = 0; j < 2; j++) acc[i][j] = general_mma(lb + (wn + 16 * j) * P, la + (wm + 16 * i) * P, acc[i][j]);
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 2; i++)
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int64_t m = m0 + wm + 16 * i + (l & 15), n = n0 + wn + 16 * j + 4 * (l >> 4) + e;
-        if (m < g.m && n < g.n) epilogue(g, m, n, acc[i][j][e]);
-      }
-}
-
-// ---- the splits of K joined: eight columns a thread, splits in order -----------------------------------------------------
+// ---- the splits of K joined: eight columns a thread, splits in order.  The loads of up to eight splits are under way at once
+// (one after the other their latency made 9 us of 16 splits of 24 x 1024; so 4).
 template <typename T>
-__global__ __launch_bounds__(256) void join_splits_kernel(Gemm<T> g, const float *partial, int splits, int64_t per_row) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, m = i / per_row, n = i % per_row * 8;
+__global__ __launch_bounds__(256) void join_splits_kernel(Gemm<T> g, const float *partial, int splits, uint32_t per_row) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  int64_t m, n;
+  if (i >> 32) m = i / per_row, n = i % per_row * 8;
+  else m = (uint32_t)i / per_row, n = ((uint32_t)i - (uint32_t)m * per_row) * 8;
   if (m >= g.m) return;
   Columns c;
   c.load(g, n);
-  const bool whole = n + 8 <= g.n && (g.n & 3) == 0;
+  const int64_t pitch = part_pitch(g.n), step = g.m * pitch;
+  const float *p = partial + m * pitch + n;
   f32x4 lo = {}, hi = {};
-  for (int s = 0; s < splits; s++) {
-    const float *p = partial + ((int64_t)s * g.m + m) * g.n + n;
-    if (whole) {
-      lo += *(const f32x4 *)p;
-      hi += *(const f32x4 *)(p + 4);
-    } else {
+  for (int s0 = 0; s0 < splits; s0 += 8) {
+    f32x4 a[8], b[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (n + e < g.n) {
-          if (e < 4) lo[e] += p[e];
-          else hi[e - 4] += p[e];
-        }
-    }
+    for (int s = 0; s < 8; s++)
+      if (s0 + s < splits) {
+        a[s] = *(const f32x4 *)(p + (s0 + s) * step);
+        b[s] = *(const f32x4 *)(p + (s0 + s) * step + 4);
+      }
+#pragma unroll
+    for (int s = 0; s < 8; s++)
+      if (s0 + s < splits) lo += a[s], hi += b[s];
   }
   epilogue8(g, c, m, n, lo, hi);
 }
@@ -105,52 +41,46 @@ template <typename T>
 int join_splits(const Gemm<T> &g, const float *partial, int splits, hipStream_t stream) {
   const int64_t per_row = (g.n + 7) / 8, blocks = (g.m * per_row + 255) / 256;
   if (blocks > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many blocks");
-  join_splits_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(g, partial, splits, per_row);
+  join_splits_kernel<T><<<(unsigned)blocks, 256, 0, stream>>>(g, partial, splits, (uint32_t)per_row);
   OBB_LAUNCH_CHECK();
   return OBB_OK;
 }
 
-Plan plan16(int64_t m, int64_t n, int64_t k) {
+// A product is cut by the cheapest of: rounds that the device needs x slabs of a workgroup x the time of a slab (by how many
+// workgroups share a CU), plus the splits' sums written and read back (at 4.7 TB/s) and the launch that joins them.
+struct Cut { int tile, rows, cols, fit; double slab[4]; };     // slab[i]: us of 64 k (fp32: 32 k) with i + 1 workgroups on a CU
+static Plan cheapest(const Cut *cuts, int count, int64_t m, int64_t n, int64_t slabs) {
   const int force = (int)tuning(OBB_TUNE_LINEAR_TILE, 0), force_s = (int)tuning(OBB_TUNE_LINEAR_SPLITS, 0);
-  // The cheapest by: rounds the device needs x slabs of a workgroup x the time of a slab (by how many workgroups share a CU),
-  // plus the splits' sums written and read back (at 4.7 TB/s) and the launch that joins them.
-  // Measured at 2000 x 12544 x 1024 bf16: 256 / 8 splits 64 us, 128 / 4 69, 128 / 2 81, 64 / 1 85, 128 / 1 137, 256 / 1 229;
-  // at 2000 x 1024 x 1024: 64 / 1 17, 128 / 1 18, with 2 splits 23.
-  const int64_t slabs = (k + 63) / 64;
-  Plan best = {64, 1};
+  Plan best = {cuts[count - 1].tile, 1};
   double least = 1e30;
-  for (int tile : {256, 128, 64}) {
-    if (force && tile != force) continue;
-    const int64_t tiles = ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
-    const int fit = tile == 256 ? 1 : tile == 128 ? 2 : 4;
+  for (int i = 0; i < count; i++) {
+    const Cut &c = cuts[i];
+    if (force && c.tile != force) continue;
+    const int64_t tiles = ((m + c.rows - 1) / c.rows) * ((n + c.cols - 1) / c.cols);
     for (int s = 1; s <= 16 && (s == 1 || s * 2 <= slabs); s *= 2) {
       if (force_s && s != force_s) continue;
-      const int64_t per_cu = (tiles * s + 255) / 256, rounds = (per_cu + fit - 1) / fit;
-      const int share = per_cu < fit ? (int)per_cu : fit;
-      const double slab = tile == 256 ? 1.4 : tile == 128 ? (share == 1 ? 0.66 : 1.0) : (share == 1 ? 0.36 : share == 2 ? 0.43 : 0.75);
-      double us = 3.0 + rounds * (2.0 + slab * ((slabs + s - 1) / s));
-      if (s > 1) us += 4.0 + 2.0 * s * m * n * 4 / 4.7e6;
-      if (us < least) least = us, best = {tile, s};
+      const int64_t per_cu = (tiles * s + 255) / 256, rounds = (per_cu + c.fit - 1) / c.fit;
+      const int share = per_cu < c.fit ? (int)per_cu : c.fit;
+      double us = 3.0 + rounds * (2.0 + c.slab[share > 0 ? share - 1 : 0] * ((slabs + s - 1) / s));
+      if (s > 1) us += 3.0 + 2.0 * s * m * n * 4 / 4.7e6;
+      if (us < least) least = us, best = {c.tile, s};
     }
   }
   return best;
 }
 
-// The same for fp32 (steps of 32 k, 128 x 128 tiles, two workgroups on a CU).  Measured at 2000 x 12544 x 1024: 4 splits 262 us,
-// 2 splits 291, none 503.
+// Measured, us, tile / splits: 2000 x 12544 x 1024 bf16 256 / 8 64, 256 x 128 / 4 59, 128 / 4 69, 64 / 1 85, 256 / 1 226;
+// 1024 x 12544 x 1024 256 / 8 50, 256 x 128 / 8 38, 128 / 8 43; 4096^3 256 / 1 106, 256 x 128 / 1 125; 777 x 1112 x 520 64 / 1 10, 128 / 1 20.
+Plan plan16(int64_t m, int64_t n, int64_t k) {
+  static const Cut cuts[] = {{256, 256, 256, 1, {1.25}}, {192, 256, 128, 1, {0.8}}, {128, 128, 128, 2, {0.76, 1.0}}, {64, 64, 64, 4, {0.36, 0.43, 0.6, 0.75}}};
+  return cheapest(cuts, 4, m, n, (k + 63) / 64);
+}
+
+// Measured, us, tile / splits: 2000 x 12544 x 1024 fp32 128 / 4 258, 128 / 2 279, 64 / 1 355; 4096^3 128 / 1 627, 64 / 1 843;
+// 777 x 1111 x 515 64 / 4 19, 64 / 1 28, 128 / 4 24, 128 / 1 65.
 Plan plan32(int64_t m, int64_t n, int64_t k) {
-  const int force_s = (int)tuning(OBB_TUNE_LINEAR_SPLITS, 0);
-  const int64_t steps = (k + 31) / 32, tiles = ((m + 127) / 128) * ((n + 127) / 128);
-  Plan best = {128, 1};
-  double least = 1e30;
-  for (int s = 1; s <= 16 && (s == 1 || s * 4 <= steps); s *= 2) {
-    if (force_s && s != force_s) continue;
-    const int64_t per_cu = (tiles * s + 255) / 256, rounds = (per_cu + 1) / 2;
-    double us = 3.0 + rounds * (2.0 + (per_cu == 1 ? 1.35 : 2.47) * ((steps + s - 1) / s));
-    if (s > 1) us += 4.0 + 2.0 * s * m * n * 4 / 4.7e6;
-    if (us < least) least = us, best.splits = s;
-  }
-  return best;
+  static const Cut cuts[] = {{128, 128, 128, 2, {1.3, 2.42}}, {64, 64, 64, 3, {0.62, 0.9, 1.15}}};
+  return cheapest(cuts, 2, m, n, (k + 31) / 32);
 }
 
 static bool aligned16(const void *p, int64_t ld, int64_t extent) {
@@ -160,70 +90,131 @@ static bool aligned16(const void *p, int64_t ld, int64_t extent) {
 template <typename T, bool TA, bool TB>
 int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
   if (g.m == 0 || g.n == 0) return OBB_OK;
-  if constexpr (sizeof(T) == 2) {
-    // (a workgroup's slab must fit a buffer descriptor: 256 rows, or 64 when the contraction is outermost, below 2 GiB)
-    if (aligned16(g.a, g.lda, TA ? g.m : g.k) && aligned16(g.b, g.ldb, TB ? g.n : g.k) && g.lda < (1 << 22) - 256 && g.ldb < (1 << 22) - 256) {
-      const Plan p = plan16(g.m, g.n, g.k);
-      if (int rc = gemm_mfma<T, TA, TB>(g, p.tile, p.splits, ws, stream)) return rc;
-      return p.splits > 1 ? join_splits(g, ws, p.splits, stream) : OBB_OK;
-    }
-    if (tuning(OBB_TUNE_LINEAR_TILE, 0) != 1) {
-      // (the same splits: the workspace is sized without looking at pointers)
-      const Plan p = plan16(g.m, g.n, g.k);
-      if (int rc = gemm_ragged<T, TA, TB>(g, p.tile, p.splits, ws, stream)) return rc;
-      return p.splits > 1 ? join_splits(g, ws, p.splits, stream) : OBB_OK;
-    }
-  }
+  Plan p;
+  int rc;
   if constexpr (sizeof(T) == 4) {
-    if (tuning(OBB_TUNE_LINEAR_TILE, 0) != 1) {
-      const Plan p = plan32(g.m, g.n, g.k);
-      if (int rc = gemm_split<TA, TB>(g, p.tile, p.splits, ws, stream)) return rc;
-      return p.splits > 1 ? join_splits(g, ws, p.splits, stream) : OBB_OK;
-    }
+    p = plan32(g.m, g.n, g.k);
+    rc = gemm_split<TA, TB>(g, p.tile, p.splits, ws, stream);
+  } else {
+    p = plan16(g.m, g.n, g.k);      // (the same for both kernels: the workspace is sized without looking at pointers)
+    // Direct loads need 16-byte chunks that end with the operand, and a slab that fits a buffer descriptor: 256 rows, or 64
+    // where the contraction is outermost, below 2 GiB.  (4096^3 bf16: 105 us; 4095^3 through registers 250.)
+    if (aligned16(g.a, g.lda, TA ? g.m : g.k) && aligned16(g.b, g.ldb, TB ? g.n : g.k) && g.lda < (1 << 22) - 256 && g.ldb < (1 << 22) - 256)
+      rc = gemm_mfma<T, TA, TB>(g, p.tile, p.splits, ws, stream);
+    else
+      rc = gemm_ragged<T, TA, TB>(g, p.tile, p.splits, ws, stream);
   }
-  const int64_t tm = (g.m + GT - 1) / GT, tn = (g.n + GT - 1) / GT;
-  if (tm * tn > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many tiles (%lld x %lld)", (long long)tm, (long long)tn);
-  gemm_general_kernel<T, TA, TB><<<(unsigned)(tm * tn), 256, 0, stream>>>(g, tn);
-  OBB_LAUNCH_CHECK();
-  return OBB_OK;
+  return rc ? rc : p.splits > 1 ? join_splits(g, ws, p.splits, stream) : OBB_OK;
 }
 
 // ---- dz = dy act'(z) and db = sum_m dz: one pass over dy, column sums in two fixed steps (no atomics: the same bits
-// every run).  Block (x, y): 64 columns, rows y, y + chunks, ... of 64; partial sums [chunk][n] in the workspace.
+// every run).  Block (x, y): 64 columns, rows y, y + chunks, ... of CS_ROWS; 16-byte accesses where the rows are aligned, four rows
+// under way a thread; partial sums [chunk][n] in the workspace.
 constexpr int CS_COLS = 64;
-static int colsum_chunks(int64_t m, int64_t n) {
-  const int64_t want = 2048 / ((n + CS_COLS - 1) / CS_COLS) + 1, have = (m + 63) / 64;
+template <typename T> constexpr int cs_rows() { return 256 / (CS_COLS * (int)sizeof(T) / 16) * 4; }     // rows a block takes at once
+static int colsum_chunks(int64_t m, int64_t n, int dtype) {
+  const int rows = dtype == OBB_F32 ? cs_rows<float>() : cs_rows<__bf16>();
+  const int64_t want = 4096 / ((n + CS_COLS - 1) / CS_COLS) + 1, have = (m + rows - 1) / rows;
   return (int)(want < have ? want : (have < 1 ? 1 : have));
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void act_backward_kernel(const T *dy, const T *y, const float *z, int64_t m, int64_t n, int act,
-                                                           T *dz, float *partial) {
-  __shared__ float sums[4][CS_COLS];
-  const int c = threadIdx.x & 63, r = threadIdx.x >> 6;
-  const int64_t col = (int64_t)blockIdx.x * CS_COLS + c;
-  float sum = 0.f;
-  if (col < n)
-    for (int64_t row = (int64_t)blockIdx.y * 4 + r; row < m; row += (int64_t)gridDim.y * 4) {
-      const int64_t at = row * n + col;
-      float v = to_f32(dy[at]);
-      if (act != OBB_ACT_NONE) v *= act_slope(act == OBB_ACT_RELU ? to_f32(y[at]) : z[at], act);
-      sum += v;
-      if (dz) dz[at] = from_f32<T>(v);
+                                                           T *dz, float *partial, bool aligned) {
+  constexpr int W = 16 / sizeof(T), G = CS_COLS / W, RP = 256 / G;      // columns a thread, threads a row, rows a pass
+  typedef T tw __attribute__((ext_vector_type(W)));
+  __shared__ float sums[RP][CS_COLS + 1];
+  const int c = threadIdx.x % G, r = threadIdx.x / G;
+  const int64_t col = (int64_t)blockIdx.x * CS_COLS + c * W;
+  const bool whole = aligned && col + W <= n;
+  float sum[W] = {};
+  for (int64_t r0 = (int64_t)blockIdx.y * (4 * RP); r0 < m; r0 += (int64_t)gridDim.y * (4 * RP)) {
+    float d[4][W], v[4][W];
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int64_t row = r0 + q * RP + r, at = row * n + col;
+#pragma unroll
+      for (int e = 0; e < W; e++) d[q][e] = 0.f, v[q][e] = 0.f;
+      if (row < m && whole) {
+        const tw t = *(const tw *)(dy + at);
+#pragma unroll
+        for (int e = 0; e < W; e++) d[q][e] = to_f32((T)t[e]);
+        if (act == OBB_ACT_RELU) {
+          const tw u = *(const tw *)(y + at);
+#pragma unroll
+          for (int e = 0; e < W; e++) v[q][e] = to_f32((T)u[e]);
+        } else if (act != OBB_ACT_NONE) {
+#pragma unroll
+          for (int e = 0; e < W; e += 4) {
+            const f32x4 u = *(const f32x4 *)(z + at + e);
+            v[q][e] = u[0], v[q][e + 1] = u[1], v[q][e + 2] = u[2], v[q][e + 3] = u[3];
+          }
+        }
+      } else if (row < m) {
+#pragma unroll
+        for (int e = 0; e < W; e++)
+          if (col + e < n) {
+            d[q][e] = to_f32(dy[at + e]);
+            if (act != OBB_ACT_NONE) v[q][e] = act == OBB_ACT_RELU ? to_f32(y[at + e]) : z[at + e];
+          }
+      }
     }
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      const int64_t row = r0 + q * RP + r, at = row * n + col;
+      if (row >= m) continue;
+      if (act != OBB_ACT_NONE)
+#pragma unroll
+        for (int e = 0; e < W; e++) d[q][e] *= act_slope(v[q][e], act);
+#pragma unroll
+      for (int e = 0; e < W; e++) sum[e] += d[q][e];
+      if (dz && whole) {
+        tw t;
+#pragma unroll
+        for (int e = 0; e < W; e++) t[e] = from_f32<T>(d[q][e]);
+        *(tw *)(dz + at) = t;
+      } else if (dz) {
+#pragma unroll
+        for (int e = 0; e < W; e++)
+          if (col + e < n) dz[at + e] = from_f32<T>(d[q][e]);
+      }
+    }
+  }
   if (!partial) return;
-  sums[r][c] = sum;
+#pragma unroll
+  for (int e = 0; e < W; e++) sums[r][c * W + e] = sum[e];
   __syncthreads();
-  if (r == 0 && col < n) partial[(int64_t)blockIdx.y * n + col] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+  const int64_t out = (int64_t)blockIdx.x * CS_COLS + threadIdx.x;
+  if (threadIdx.x < CS_COLS && out < n) {
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < RP; q++) s += sums[q][threadIdx.x];
+    partial[(int64_t)blockIdx.y * n + out] = s;
+  }
 }
 
+// 64 columns a block, a quarter of the chunks a wave, then the four in order
 template <typename T>
 __global__ __launch_bounds__(256) void colsum_join_kernel(const float *partial, int chunks, int64_t n, T *db) {
-  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (col >= n) return;
+  __shared__ float sums[4][64];
+  const int w = threadIdx.x >> 6, l = threadIdx.x & 63, per = (chunks + 3) / 4;
+  const int64_t col = (int64_t)blockIdx.x * 64 + l;
   float s = 0.f;
-  for (int c = 0; c < chunks; c++) s += partial[(int64_t)c * n + col];
-  db[col] = from_f32<T>(s);
+  if (col < n) {
+    const int end = (w + 1) * per < chunks ? (w + 1) * per : chunks;
+    int c = w * per;
+    for (; c + 8 <= end; c += 8) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; q++) v[q] = partial[(int64_t)(c + q) * n + col];
+#pragma unroll
+      for (int q = 0; q < 8; q++) s += v[q];
+    }
+    for (; c < end; c++) s += partial[(int64_t)c * n + col];
+  }
+  sums[w][l] = s;
+  __syncthreads();
+  if (w == 0 && col < n) db[col] = from_f32<T>((sums[0][l] + sums[1][l]) + (sums[2][l] + sums[3][l]));
 }
 
 static bool bad_dtype(int d) { return d != OBB_F32 && d != OBB_BF16 && d != OBB_F16; }
@@ -232,13 +223,14 @@ static bool bad_act(int a) { return a < OBB_ACT_NONE || a > OBB_ACT_SILU; }
 template <typename T>
 static int act_backward(const void *dy, const void *y, const float *z, int64_t m, int64_t n, int act, void *dz, void *db,
                         void *ws, hipStream_t stream) {
-  const int chunks = colsum_chunks(m, n);
+  const int chunks = colsum_chunks(m, n, sizeof(T) == 4 ? OBB_F32 : OBB_BF16);
   float *partial = db ? (float *)ws : nullptr;
+  const bool aligned = n * sizeof(T) % 16 == 0 && (((uintptr_t)dy | (uintptr_t)y | (uintptr_t)z | (uintptr_t)dz) & 15) == 0;
   act_backward_kernel<T><<<dim3((unsigned)((n + CS_COLS - 1) / CS_COLS), chunks), 256, 0, stream>>>(
-      (const T *)dy, (const T *)y, z, m, n, act, (T *)dz, partial);
+      (const T *)dy, (const T *)y, z, m, n, act, (T *)dz, partial, aligned);
   OBB_LAUNCH_CHECK();
   if (db) {
-    colsum_join_kernel<T><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(partial, chunks, n, (T *)db);
+    colsum_join_kernel<T><<<(unsigned)((n + 63) / 64), 256, 0, stream>>>(partial, chunks, n, (T *)db);
     OBB_LAUNCH_CHECK();
   }
   return OBB_OK;
@@ -269,11 +261,11 @@ using namespace obb::lin;
 
 extern "C" size_t obb_linear_workspace_bytes(int64_t m, int64_t n, int64_t k, int dtype, int op) {
   if (m < 0 || n < 0 || k < 0 || bad_dtype(dtype)) return 0;
-  if (op == OBB_LINEAR_ACT_BACKWARD) return align_up((size_t)colsum_chunks(m, n) * (size_t)n * 4, 256);
+  if (op == OBB_LINEAR_ACT_BACKWARD) return align_up((size_t)colsum_chunks(m, n, dtype) * (size_t)n * 4, 256);
   if (op == OBB_LINEAR_BACKWARD_INPUT) std::swap(n, k);            // (m, k) = (m, n) (n, k)
   if (op == OBB_LINEAR_BACKWARD_WEIGHT) { const int64_t t = m; m = n; n = k; k = t; }   // (n, k) = (n, m) (m, k)
   const Plan p = dtype == OBB_F32 ? plan32(m, n, k) : plan16(m, n, k);
-  return p.splits > 1 ? align_up((size_t)p.splits * (size_t)m * (size_t)n * 4, 256) : 0;
+  return p.splits > 1 ? align_up((size_t)p.splits * (size_t)m * (size_t)part_pitch(n) * 4, 256) : 0;
 }
 
 extern "C" int obb_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, const void *res,

@@ -152,15 +152,9 @@ __device__ __forceinline__ void epilogue4(const Gemm<T> &g, int64_t m, int64_t n
   *(t4 *)(g.y + at) = out;
 }
 
-// the sums of one split, (m, n) fp32 in the workspace; `whole`: rows are multiples of four columns
-__device__ __forceinline__ void store4_partial(float *p, int64_t cols, int64_t m, int64_t n, f32x4 v, bool whole) {
-  float *at = p + m * cols + n;
-  if (whole) *(f32x4 *)at = v;
-  else
-#pragma unroll
-    for (int e = 0; e < 4; e++)
-      if (n + e < cols) at[e] = v[e];
-}
+// the sums of one split, (m, n) fp32 in the workspace with rows of a multiple of eight columns (the padding holds whatever the
+// tile's sums beyond the edge are)
+__host__ __device__ __forceinline__ int64_t part_pitch(int64_t n) { return (n + 7) & ~(int64_t)7; }
 
 // Workgroup number -> tile.  Workgroups go to the 8 dies in turn: the number is turned so that a die gets a run of tiles, and
 // the runs walk blocks of 8 tile rows, so that the tiles a die works on at a time share rows of both operands in its L2.
@@ -180,13 +174,13 @@ template <typename T, int ACT, int FM, int FN>
 __device__ __forceinline__ void tile_out(const Gemm<T> &g, const f32x4 (&acc)[FM][FN], int64_t m0, int64_t n0, float *part, float *mine, int lane) {
   const int64_t nw = n0 + 4 * (lane >> 4);      // of the lane's four columns in fragment j: + 16 j
   if (part) {
-    const bool whole = (g.n & 3) == 0;
+    const int64_t pitch = part_pitch(g.n);
 #pragma unroll
     for (int i = 0; i < FM; i++) {
       const int64_t m = m0 + 16 * i + (lane & 15);
 #pragma unroll
       for (int j = 0; j < FN; j++)
-        if (m < g.m && nw + 16 * j < g.n) store4_partial(part, g.n, m, nw + 16 * j, acc[i][j], whole);
+        if (m < g.m && nw + 16 * j < pitch) *(f32x4 *)(part + m * pitch + nw + 16 * j) = acc[i][j];
     }
     return;
   }

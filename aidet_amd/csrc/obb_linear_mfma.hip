@@ -1,7 +1,7 @@
 // obb_linear_mfma.hip -- the tiled product of 16-bit operands: C (M, N) = sum_k A(m, k) B(n, k), epilogue of the fused
 // linear layer, either operand stored with its contraction innermost ("rows") or outermost ("columns").
 //
-// A workgroup owns a BM x BN tile and walks K in steps of 32 through a ring of five LDS slots: memory -> LDS without registers
+// A workgroup owns a BM x BN tile and walks K in steps of 32 through LDS slots, three per operand (two for the second where LDS ends): memory -> LDS without registers
 // in between (buffer loads that write LDS), LDS -> fragments one step ahead, fragments -> matrix instructions.  One barrier a
 // step: behind it the slot whose fragments everybody has taken is filled again, four steps before it is needed.
 // What bounds it: the matrix pipe, once the loads' latency is covered.  With two slots of 64 k (one in flight at a time) the
@@ -15,12 +15,14 @@
 //
 // Edges: a lane whose chunk lies outside the operand reads at an offset beyond the buffer descriptor's size, which gives
 // zeros; a chunk never straddles an edge, because the caller has checked that the contiguous extent is a multiple of 8.
+#include <type_traits>
+
 #include "obb_linear_internal.h"
 
 namespace obb {
 namespace lin {
 
-constexpr int BK = 64, RING = 5;
+constexpr int BK = 64;
 
 
 template <typename T> struct Vec8;
@@ -116,10 +118,9 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, uint3
   constexpr int WAVES = WM * WN, FM = BM / WM / 16, FN = BN / WN / 16;
   typedef Slab<T, BM, WAVES, TA> SA;
   typedef Slab<T, BN, WAVES, TB> SB;
-  static_assert(BM == BN, "slots serve either operand");
-  constexpr uint32_t SLOT = SA::BYTES;
-  constexpr int LOADS = SA::LOADS + SB::LOADS;
-  __shared__ __attribute__((aligned(1024))) char lds[RING * SLOT];
+  // LDS slots: three for A, and two for B where three would take the workgroup more than its share of a CU's LDS
+  constexpr uint32_t DA = 3, DB = BM == BN ? 2 : 3, A_BYTES = DA * SA::BYTES;
+  __shared__ __attribute__((aligned(1024))) char lds[A_BYTES + DB * SB::BYTES];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
   const uint32_t split = blockIdx.x % splits;
@@ -146,12 +147,13 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, uint3
   // a wave issues in order, and loads in a row would hold back its matrix instructions while the address unit (16 cycles
   // a load, all waves') is busy.
   auto half = [&](int h, uint32_t at_a, uint32_t at_b, const auto &s, int64_t t, uint32_t to) {
-    constexpr int Q = SA::LOADS, R = (FM + FN + Q - 1) / Q;
+    constexpr int Q = std::remove_reference_t<decltype(s)>::LOADS < FM ? std::remove_reference_t<decltype(s)>::LOADS : FM, R = (FM + FN + Q - 1) / Q, P = std::remove_reference_t<decltype(s)>::LOADS / Q;
 #pragma unroll
     for (int q = 0; q < Q; q++) {
 #pragma unroll
       for (int f = q * R; f < q * R + R && f < FM + FN; f++) read(f, h ^ 1, at_a, at_b);
-      s.issue(q, t, kk - t * BK, lds0 + to, wave);
+#pragma unroll
+      for (int i = q * P; i < q * P + P; i++) s.issue(i, t, kk - t * BK, lds0 + to, wave);
 #pragma unroll
       for (int i = q * FM / Q; i < (q + 1) * FM / Q; i++)
 #pragma unroll
@@ -159,29 +161,31 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, uint3
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // Slots in turn: A 0, B 0, A 1, B 1, A 2, then B 2 where A 0 was, ...  (past the last slab every lane is outside and the
-  // loads give zeros: no branch in the loop)
+  // (past the last slab every lane is outside and the loads give zeros: no branch in the loop)
   if (slabs > 0) {
-    auto after = [](uint32_t at) { return at + SLOT == RING * SLOT ? 0 : at + SLOT; };
+    auto after_a = [](uint32_t at) { return at + SA::BYTES == A_BYTES ? 0 : at + SA::BYTES; };
+    auto after_b = [](uint32_t at) { return at + SB::BYTES == A_BYTES + DB * SB::BYTES ? A_BYTES : at + SB::BYTES; };
     sa.issue(0, kk, lds0, wave);
-    sb.issue(0, kk, lds0 + SLOT, wave);
-    sa.issue(1, kk - BK, lds0 + 2 * SLOT, wave);
-    sb.issue(1, kk - BK, lds0 + 3 * SLOT, wave);
-    wait_and_meet<SA::LOADS + SB::LOADS>();
-    uint32_t at_a = 0, at_b = SLOT, free_slot = 4 * SLOT;
+    sb.issue(0, kk, lds0 + A_BYTES, wave);
+    sa.issue(1, kk - BK, lds0 + SA::BYTES, wave);
+    sb.issue(1, kk - BK, lds0 + A_BYTES + SB::BYTES, wave);
+    if (DB == 3) sb.issue(2, kk - 2 * BK, lds0 + A_BYTES + 2 * SB::BYTES, wave);
+    wait_and_meet<SA::LOADS + (DB - 1) * SB::LOADS>();
+    uint32_t at_a = 0, at_b = A_BYTES, free_a = 2 * SA::BYTES;
 #pragma unroll
     for (int f = 0; f < FM + FN; f++) read(f, 0, at_a, at_b);
     for (int64_t t = 0; t < slabs; t++) {
-      half(0, at_a, at_b, sa, t + 2, free_slot);   // (where B t - 1 was)
-      wait_and_meet<SA::LOADS>();                  // A, B t + 1 have landed, everybody has slab t's fragments
-      const uint32_t to = at_a;
-      free_slot = at_b;
-      at_a = after(at_b), at_b = after(at_a);
-      half(1, at_a, at_b, sb, t + 2, to);
+      half(0, at_a, at_b, sa, t + 2, free_a);                       // (where A t - 1 was)
+      // A, B t + 1 have landed -- behind them A t + 2 and, with three slots, B t + 2 are on the way -- and everybody has slab t's fragments
+      wait_and_meet<SA::LOADS + (DB - 2) * SB::LOADS>();
+      const uint32_t to = at_b;
+      free_a = at_a;
+      at_a = after_a(at_a), at_b = after_b(at_b);
+      half(1, at_a, at_b, sb, t + DB, to);
     }
   }
   wait_and_meet<0>();
-  tile_out<T, ACT, FM, FN>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * g.n : nullptr, (float *)lds + wave * 256 * FN, lane);
+  tile_out<T, ACT, FM, FN>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, (float *)lds + wave * 256 * FN, lane);
 }
 
 // ---- the same product where rows or edges are not aligned: through registers ----------------------------------------------
@@ -293,7 +297,7 @@ __global__ __launch_bounds__(256) void gemm_ragged_kernel(Gemm<T> g, uint32_t ti
     }
     __syncthreads();
   }
-  tile_out<T, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * g.n : nullptr, (float *)lds + wave * 256 * F, lane);
+  tile_out<T, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, (float *)lds + wave * 256 * F, lane);
 }
 
 template <typename T, int B, bool TA, bool TB>
@@ -341,6 +345,7 @@ static int launch(const Gemm<T> &g, int splits, float *partial, hipStream_t stre
 template <typename T, bool TA, bool TB>
 int gemm_mfma(const Gemm<T> &g, int tile, int splits, float *partial, hipStream_t stream) {
   if (tile == 256) return launch<T, 256, 256, 2, 4, TA, TB>(g, splits, partial, stream);
+  if (tile == 192) return launch<T, 256, 128, 4, 2, TA, TB>(g, splits, partial, stream);     // (by its mean edge)
   if (tile == 128) return launch<T, 128, 128, 2, 2, TA, TB>(g, splits, partial, stream);
   return launch<T, 64, 64, 2, 2, TA, TB>(g, splits, partial, stream);
 }

@@ -56,14 +56,19 @@ struct Stage {
   int64_t ld;
   int rows;            // rows of the tile that exist (rows beyond repeat one of them: their outputs are not stored)
   const float *row[N]; // "rows": the thread's chunk of step 0
-  int at[N / 2];       // "columns": the thread's first row of two; the operand's last pair where that one lies outside
-  bool odd[N / 2];     // ... and its row is that pair's second
+  // "columns": the thread's first row of two; the operand's last pair where that one lies outside, and then it is that pair's
+  // second.  64 rows: one row.
+  static constexpr int PAIRS = N > 1 ? N / 2 : 1;
+  int at[PAIRS];
+  bool odd[PAIRS];
 
   __device__ __forceinline__ void init(const float *p, int64_t pitch, int64_t r0, int64_t all, int64_t k0) {
     base = p + (TR ? k0 * pitch + r0 : r0 * pitch + k0);
     ld = pitch;
     rows = all - r0 < R ? (int)(all - r0) : R;
-    if constexpr (TR) {
+    if constexpr (TR && N == 1) {
+      at[0] = (int)(threadIdx.x & 63) < rows ? (int)(threadIdx.x & 63) : rows - 1;
+    } else if constexpr (TR) {
 #pragma unroll
       for (int i = 0; i < N / 2; i++) {
         const int r = 2 * (int)(threadIdx.x & 63) + 128 * i;
@@ -78,11 +83,19 @@ struct Stage {
       }
     }
   }
+  // the thread's row i
+  __device__ __forceinline__ static int row_of(int i) {
+    return !TR ? (int)(threadIdx.x >> 2) + 64 * i : N == 1 ? (int)(threadIdx.x & 63) : 2 * (int)(threadIdx.x & 63) + 128 * (i / 2) + (i & 1);
+  }
   // whether load_whole() stays inside
-  __device__ __forceinline__ bool pairs() const { return !TR || rows > 1; }
+  __device__ __forceinline__ bool pairs() const { return !TR || N == 1 || rows > 1; }
   // rows 0 ... i (of which load i brings those not there yet) of step t, all of its k inside
   __device__ __forceinline__ void load_whole(int i, int64_t t) {
-    if constexpr (TR) {
+    if constexpr (TR && N == 1) {
+      const float *p = base + (t * BK + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 8) * ld;
+#pragma unroll
+      for (int k = 0; k < 8; k++, p += ld) x[0][k] = p[at[0]];
+    } else if constexpr (TR) {
       if (i & 1) {
         const float *p = base + (t * BK + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 8) * ld;
 #pragma unroll
@@ -108,7 +121,7 @@ struct Stage {
     const int k0 = 8 * (int)(TR ? threadIdx.x >> 6 : threadIdx.x & 3);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-      int r = TR ? 2 * (int)(threadIdx.x & 63) + 128 * (i / 2) + (i & 1) : (int)(threadIdx.x >> 2) + 64 * i;
+      int r = row_of(i);
       r = r < rows ? r : rows - 1;
       const float *q = TR ? base + t * BK * ld + r : base + r * ld + t * BK;
 #pragma unroll
@@ -120,7 +133,7 @@ struct Stage {
     }
   }
   __device__ __forceinline__ void store(int i, char *lds) const {        // row i into three planes of R * 64 bytes
-    const int r = TR ? 2 * (int)(threadIdx.x & 63) + 128 * (i / 2) + (i & 1) : (int)(threadIdx.x >> 2) + 64 * i;
+    const int r = row_of(i);
     const int c = TR ? (int)(threadIdx.x >> 6) : (int)(threadIdx.x & 3);
     const Parts p = split8(x[i]);
     char *to = lds + place(r, c);
@@ -134,15 +147,15 @@ struct Stage {
   }
 };
 
-// A 128 x 128 tile on four waves of 64 x 64.  A step: everybody takes the fragments of three planes of both operands from LDS;
+// A B x B tile (128 or 64) on four waves of half its edge.  A step: everybody takes the fragments of three planes of both operands from LDS;
 // behind a barrier the next step's numbers are split and written there, the step after next is requested from memory, and the
 // 96 matrix instructions run.  Two workgroups share a CU: one splits while the other multiplies.
-template <bool TA, bool TB, int ACT>
-__global__ __launch_bounds__(256, 2) void gemm_split_kernel(Gemm<float> g, uint32_t tiles_m, uint32_t tiles_n, uint32_t splits, int64_t per, float *partial) {
-  constexpr int B = 128, F = 4;
+template <int B, bool TA, bool TB, int ACT>
+__global__ __launch_bounds__(256, B == 128 ? 2 : 3) void gemm_split_kernel(Gemm<float> g, uint32_t tiles_m, uint32_t tiles_n, uint32_t splits, int64_t per, float *partial) {
+  constexpr int F = B / 32;
   __shared__ __attribute__((aligned(128))) char lds[2 * 3 * B * 64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int wm = wave / 2 * 64, wn = wave % 2 * 64;
+  const int wm = wave / 2 * (B / 2), wn = wave % 2 * (B / 2);
   const uint32_t split = blockIdx.x % splits;
   uint32_t tm, tn;
   tile_of(blockIdx.x / splits, tiles_m, tiles_n, tm, tn);
@@ -172,14 +185,15 @@ __global__ __launch_bounds__(256, 2) void gemm_split_kernel(Gemm<float> g, uint3
           fb[p][i] = *(const bf16x8 *)(lb + p * B * 64 + place(wn + 16 * i + (lane & 15), lane >> 4));
         }
       __syncthreads();
-      // the small products first; a quarter of the next step's work before every quarter of them
+      // the small products first; the next step's work is dealt between them
       constexpr int PA[6] = {0, 1, 2, 0, 1, 0}, PB[6] = {2, 1, 0, 1, 0, 0};
 #pragma unroll
-      for (int q = 0; q < 4; q++) {
+      for (int q = 0; q < F; q++) {
         next(q);
+        constexpr int PER = 6 * F;
 #pragma unroll
-        for (int e = q * 24; e < q * 24 + 24; e++) {
-          const int p = e / 16, i = e / 4 % 4, j = e % 4;
+        for (int e = q * PER; e < q * PER + PER; e++) {
+          const int p = e / (F * F), i = e / F % F, j = e % F;
           acc[i][j] = mma(fb[PB[p]][j], fa[PA[p]][i], acc[i][j]);
         }
       }
@@ -193,12 +207,12 @@ __global__ __launch_bounds__(256, 2) void gemm_split_kernel(Gemm<float> g, uint3
     int64_t t = 0;
     for (; t + 2 < whole; t++)
       fetch_and_multiply([&](int q) {
-        if (q < 2) {
+        if (q < F / 2) {
           sa.store(q, la);
           sa.load_whole(q, t + 2);
         } else {
-          sb.store(q - 2, lb);
-          sb.load_whole(q - 2, t + 2);
+          sb.store(q - F / 2, lb);
+          sb.load_whole(q - F / 2, t + 2);
         }
       });
 #pragma unroll 1
@@ -246,24 +260,28 @@ __global__ __launch_bounds__(256, 2) void gemm_split_kernel(Gemm<float> g, uint3
           for (int e = 0; e < 4; e++) acc[i][j][e] = acc[i][j][e] != acc[i][j][e] ? ieee[i][j][e] : acc[i][j][e];
     }
   }
-  tile_out<float, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * g.n : nullptr, (float *)lds + wave * 256 * F, lane);
+  tile_out<float, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, (float *)lds + wave * 256 * F, lane);
 }
 
-template <bool TA, bool TB>
-int gemm_split(const Gemm<float> &g, int tile, int splits, float *partial, hipStream_t stream) {
-  (void)tile;
-  const int64_t tm = (g.m + 127) / 128, tn = (g.n + 127) / 128, steps = (g.k + BK - 1) / BK, per = (steps + splits - 1) / splits;
+template <int B, bool TA, bool TB>
+static int launch_split(const Gemm<float> &g, int splits, float *partial, hipStream_t stream) {
+  const int64_t tm = (g.m + B - 1) / B, tn = (g.n + B - 1) / B, steps = (g.k + BK - 1) / BK, per = (steps + splits - 1) / splits;
   if (tm * tn * splits > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many tiles (%lld x %lld)", (long long)tm, (long long)tn);
   const uint32_t grid = (uint32_t)(tm * tn * splits), um = (uint32_t)tm, un = (uint32_t)tn;
   const int act = splits > 1 ? OBB_ACT_NONE : g.act;
   if constexpr (!TA && !TB) {
-    if (act == OBB_ACT_RELU) gemm_split_kernel<TA, TB, OBB_ACT_RELU><<<grid, 256, 0, stream>>>(g, um, un, splits, per, partial);
-    if (act == OBB_ACT_GELU) gemm_split_kernel<TA, TB, OBB_ACT_GELU><<<grid, 256, 0, stream>>>(g, um, un, splits, per, partial);
-    if (act == OBB_ACT_SILU) gemm_split_kernel<TA, TB, OBB_ACT_SILU><<<grid, 256, 0, stream>>>(g, um, un, splits, per, partial);
+    if (act == OBB_ACT_RELU) gemm_split_kernel<B, TA, TB, OBB_ACT_RELU><<<grid, 256, 0, stream>>>(g, um, un, splits, per, partial);
+    if (act == OBB_ACT_GELU) gemm_split_kernel<B, TA, TB, OBB_ACT_GELU><<<grid, 256, 0, stream>>>(g, um, un, splits, per, partial);
+    if (act == OBB_ACT_SILU) gemm_split_kernel<B, TA, TB, OBB_ACT_SILU><<<grid, 256, 0, stream>>>(g, um, un, splits, per, partial);
   }
-  if (act == OBB_ACT_NONE) gemm_split_kernel<TA, TB, OBB_ACT_NONE><<<grid, 256, 0, stream>>>(g, um, un, splits, per, partial);
+  if (act == OBB_ACT_NONE) gemm_split_kernel<B, TA, TB, OBB_ACT_NONE><<<grid, 256, 0, stream>>>(g, um, un, splits, per, partial);
   OBB_LAUNCH_CHECK();
   return OBB_OK;
+}
+
+template <bool TA, bool TB>
+int gemm_split(const Gemm<float> &g, int tile, int splits, float *partial, hipStream_t stream) {
+  return tile == 64 ? launch_split<64, TA, TB>(g, splits, partial, stream) : launch_split<128, TA, TB>(g, splits, partial, stream);
 }
 
 template int gemm_split<false, false>(const Gemm<float> &, int, int, float *, hipStream_t);
