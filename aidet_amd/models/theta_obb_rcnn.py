@@ -33,6 +33,8 @@ import torch.nn.functional as F
 
 from ..anchors import AnchorGenerator
 from ..bbox_transforms import bbox2result, bbox2roi, bbox_mapping, delta2bbox
+from ..distill import topk_distill_loss
+from ..linear import fused_linear
 from ..merge_augs import merge_aug_bboxes, merge_aug_proposals
 from ..post_processing import (detect_horizontal_fused, detect_rotated_fused, get_det_rbboxes, head_fusable,
                                multiclass_nms, multiclass_nms_with_index)
@@ -49,6 +51,16 @@ TEST_CFG = dict(
                parallel=True))
 
 
+def pointwise(x, weight, bias=None, residual=None, act='none'):
+    """1 x 1 convolution of a channels-last map as one fused linear layer: every pixel is a row.  weight (N, C)."""
+    rows = None if residual is None else residual.permute(0, 2, 3, 1)
+    return fused_linear(x.permute(0, 2, 3, 1), weight, bias, rows, act).permute(0, 3, 1, 2)
+
+
+def _channels_last(x):
+    return x.is_cuda and x.is_contiguous(memory_format=torch.channels_last)
+
+
 class Bottleneck(nn.Module):
     expansion = 4
 
@@ -61,8 +73,39 @@ class Bottleneck(nn.Module):
         self.conv3 = nn.Conv2d(planes, planes * 4, 1, bias=False)
         self.bn3 = nn.BatchNorm2d(planes * 4)
         self.downsample = downsample
+        self.folded = False
+
+    # (the 1 x 1 convolutions with their frozen norm folded in; not part of the state_dict)
+    _FOLDED = ('w1', 'b1', 'w3', 'b3')
+
+    @torch.no_grad()
+    def fold(self, on=True):
+        """`on`: conv1 + bn1 + ReLU and conv3 + bn3 + shortcut + ReLU run as one fused linear layer each on channels-last maps
+        in eval mode, with the weights of NOW (loading weights, or train(), ends it)."""
+        for name in self._FOLDED:
+            self.register_buffer(name, None, persistent=False)
+        self.folded = bool(on)
+        if on:
+            for i, conv, bn in (('1', self.conv1, self.bn1), ('3', self.conv3, self.bn3)):
+                scale = bn.weight / torch.sqrt(bn.running_var + bn.eps)
+                self.register_buffer('w' + i, (conv.weight.flatten(1) * scale[:, None]).contiguous(), persistent=False)
+                self.register_buffer('b' + i, bn.bias - bn.running_mean * scale, persistent=False)
+
+    def train(self, mode=True):
+        if mode and self.folded:
+            self.fold(False)
+        return super(Bottleneck, self).train(mode)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        if self.folded:
+            self.fold(False)
+        super(Bottleneck, self)._load_from_state_dict(*args, **kwargs)
 
     def forward(self, x):
+        if self.folded and not torch.is_grad_enabled() and _channels_last(x):
+            idt = x if self.downsample is None else self.downsample(x)
+            out = F.relu(self.bn2(self.conv2(pointwise(x, self.w1, self.b1, act='relu'))), inplace=True)
+            return pointwise(out, self.w3, self.b3, idt, 'relu')
         idt = x if self.downsample is None else self.downsample(x)
         out = F.relu(self.bn1(self.conv1(x)), inplace=True)
         out = F.relu(self.bn2(self.conv2(out)), inplace=True)
@@ -105,11 +148,25 @@ class FPN(nn.Module):
         self.lateral_convs = nn.ModuleList([nn.Conv2d(c, out_channels, 1) for c in in_channels])
         self.fpn_convs = nn.ModuleList([nn.Conv2d(out_channels, out_channels, 3, padding=1) for _ in in_channels])
         self.num_outs = num_outs
+        self.fused_linear = False     # channels-last maps: a lateral and the addition of the level above as one fused linear layer
+
+    def _laterals_fused(self, inputs):
+        lat = [None] * len(inputs)
+        for i in range(len(inputs) - 1, -1, -1):
+            conv = self.lateral_convs[i]
+            up = None if lat[-1] is None else F.interpolate(lat[i + 1], size=inputs[i].shape[2:], mode='nearest')
+            lat[i] = pointwise(inputs[i], conv.weight.flatten(1), conv.bias, up)
+        return lat
 
     def forward(self, inputs):
+        if self.fused_linear and all(_channels_last(x) for x in inputs):
+            return self._outputs(self._laterals_fused(inputs))
         lat = [conv(x) for conv, x in zip(self.lateral_convs, inputs)]
         for i in range(len(lat) - 1, 0, -1):
             lat[i - 1] = lat[i - 1] + F.interpolate(lat[i], size=lat[i - 1].shape[2:], mode='nearest')
+        return self._outputs(lat)
+
+    def _outputs(self, lat):
         outs = [conv(x) for conv, x in zip(self.fpn_convs, lat)]
         while len(outs) < self.num_outs:
             outs.append(F.max_pool2d(outs[-1], 1, stride=2))
@@ -151,8 +208,9 @@ class SharedFCHead(nn.Module):
     """flatten -> FC 1024 -> ReLU -> FC 1024 -> ReLU -> fc_cls, fc_reg
     (``SharedFCBBoxHead`` with reg 4, ``RBBoxHead(num_shared_fcs=2)`` with reg 5)."""
 
-    def __init__(self, out_dim_reg, num_classes=16, in_channels=256, roi_feat_size=7, fc_out_channels=1024):
+    def __init__(self, out_dim_reg, num_classes=16, in_channels=256, roi_feat_size=7, fc_out_channels=1024, fused_linear=False):
         super(SharedFCHead, self).__init__()
+        self.fused_linear = fused_linear     # every layer one aidet_amd.fused_linear (its own kernels, differentiable) instead of F.linear + F.relu
         self.num_classes = num_classes
         self.shared_fcs = nn.ModuleList([nn.Linear(in_channels * roi_feat_size * roi_feat_size, fc_out_channels),
                                          nn.Linear(fc_out_channels, fc_out_channels)])
@@ -161,9 +219,18 @@ class SharedFCHead(nn.Module):
 
     def forward(self, x):
         x = x.flatten(1)
+        if self.fused_linear:
+            for fc in self.shared_fcs:
+                x = fused_linear(x, fc.weight, fc.bias, act='relu')
+            return fused_linear(x, self.fc_cls.weight, self.fc_cls.bias), fused_linear(x, self.fc_reg.weight, self.fc_reg.bias)
         for fc in self.shared_fcs:
             x = F.relu(fc(x))
         return self.fc_cls(x), self.fc_reg(x)
+
+    def distill_loss(self, x, teacher_values, teacher_indices, temperature=1.0, label_weights=None, avg_factor=None):
+        """Loss of this head's class logits for the pooled RoIs `x` against a teacher's top logits of the same RoIs
+        (``topk_distill_loss``); `label_weights`: those of ``rbbox_target`` (0 for a RoI that was not sampled)."""
+        return topk_distill_loss(self(x)[0], teacher_values, teacher_indices, temperature, label_weights, 'mean', avg_factor)
 
 
 def _same_extractor(a, b):
@@ -184,7 +251,7 @@ class ThetaOBBRCNN(nn.Module):
     theta-OBBs (``multiclass_rnms``).
     """
 
-    def __init__(self, test_cfg=None, rotated_nms=False, fused=True):
+    def __init__(self, test_cfg=None, rotated_nms=False, fused=True, fused_linear=False):
         super(ThetaOBBRCNN, self).__init__()
         # fused=True: the selection stages of the RPN and of both heads run as the HIP kernels of obb_detect.hip
         # (three to four launches per stage); False: the tensor-op restatement of the reference's functions, op by op
@@ -195,14 +262,14 @@ class ThetaOBBRCNN(nn.Module):
         self.rpn_head = RPNHead()
         roi = dict(type='RoIAlign', out_size=7, sample_num=2)
         self.bbox_roi_extractor = SingleRoIExtractor(roi, 256, [4, 8, 16, 32])
-        self.bbox_head = SharedFCHead(4)
+        self.bbox_head = SharedFCHead(4, fused_linear=fused_linear)
         self.rbbox_roi_extractor = SingleRoIExtractor(roi, 256, [4, 8, 16, 32])
         # Both branches pool the SAME RoIs from the same maps (test_mixins.py:281 and :352-380 call their extractors one
         # after the other); an extractor has no weights, so when the two are configured alike the second call would
         # recompute the first one's output bit for bit: at inference it is pooled once (VERDICT r3 next #3 iv: -0.35 ms
         # per tile).  `pool_once=False` keeps the reference's two calls.
         self.pool_once = True
-        self.rbbox_head = SharedFCHead(5)
+        self.rbbox_head = SharedFCHead(5, fused_linear=fused_linear)
         self.test_cfg = test_cfg or TEST_CFG
         self.rotated_nms = rotated_nms
         self.bbox_target_stds = (0.1, 0.1, 0.2, 0.2)
@@ -231,6 +298,15 @@ class ThetaOBBRCNN(nn.Module):
             nn.init.normal_(head.fc_reg.weight, 0, 0.001)
             nn.init.zeros_(head.fc_cls.bias)
             nn.init.zeros_(head.fc_reg.bias)
+
+    def fold_pointwise(self, on=True):
+        """Inference on channels-last maps: the bottlenecks' 1 x 1 convolutions (norm folded in, shortcut and ReLU in the
+        epilogue) and the FPN laterals run as fused linear layers.  Folds the weights of now: call it again after changing them."""
+        for m in self.backbone.modules():
+            if isinstance(m, Bottleneck):
+                m.fold(on)
+        self.neck.fused_linear = bool(on)
+        return self
 
     # ---- timing hooks (bench): wall time per stage, device synchronised at the boundaries ----
     def _tick(self, name):
@@ -350,9 +426,9 @@ class ThetaOBBRCNN(nn.Module):
         return bbox_results, rbbox2result(det_rbboxes, det_rlabels, self.rbbox_head.num_classes)
 
 
-def build_detector(device, rotated_nms=False, seed=0, fused=True):
+def build_detector(device, rotated_nms=False, seed=0, fused=True, fused_linear=False):
     torch.manual_seed(seed)
-    return ThetaOBBRCNN(rotated_nms=rotated_nms, fused=fused).to(device).eval()
+    return ThetaOBBRCNN(rotated_nms=rotated_nms, fused=fused, fused_linear=fused_linear).to(device).eval()
 
 
 def demo_inputs(device, size=1024, seed=0):
