@@ -457,7 +457,7 @@ static int check(const char *who, int64_t rows, int64_t classes, int64_t ld, int
   if (k > KMAX) return set_err(OBB_EINVAL, "%s: k %d > %d", who, k, KMAX);
   if (dtype < OBB_F32 || dtype > OBB_F16 || vtype < OBB_F32 || vtype > OBB_F16) return set_err(OBB_EINVAL, "%s: unknown dtype", who);
   if (itype != 4 && itype != 8) return set_err(OBB_EINVAL, "%s: an index has 4 or 8 bytes", who);
-  if (!(temperature > 0.f) || temperature > 3.0e38f) return set_err(OBB_EINVAL, "%s: temperature must be positive and finite", who);
+  if (!(temperature >= 1e-6f && temperature <= 1e6f)) return set_err(OBB_EINVAL, "%s: temperature must lie in [1e-6, 1e6]", who);   // (its square and reciprocal in fp32)
   if (rows > 1 && ld < classes) return set_err(OBB_EINVAL, "%s: row pitch below the row length", who);
   return OBB_OK;
 }
@@ -483,6 +483,7 @@ extern "C" int obb_topk_distill_forward(const void *logits, int64_t ld, int64_t 
     return set_err(OBB_EINVAL, "obb_topk_distill_forward: null pointer");
   if (ws_bytes < obb_topk_distill_workspace_bytes(rows, classes) || (!ws && ws_bytes))
     return set_err(OBB_EWORKSPACE, "obb_topk_distill_forward: workspace too small");
+  if (ws && ((uintptr_t)ws & 15)) return set_err(OBB_EINVAL, "obb_topk_distill_forward: the workspace must be 16-byte aligned");
   hipStream_t st = (hipStream_t)stream;
   Args a = {};
   a.logits = logits; a.ld = ld; a.rows = rows; a.classes = classes; a.values = values; a.indices = indices;

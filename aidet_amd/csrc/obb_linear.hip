@@ -246,6 +246,12 @@ static int check_sizes(const char *who, int64_t m, int64_t n, int64_t k, int dty
   return OBB_OK;
 }
 
+static int check_workspace(const char *who, const void *ws, size_t have, size_t need) {
+  if (have < need || (need && !ws)) return set_err(OBB_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", who, have, need);
+  if (need && ((uintptr_t)ws & 15)) return set_err(OBB_EINVAL, "%s: the workspace must be 16-byte aligned", who);
+  return OBB_OK;
+}
+
 #define OBB_LIN_DISPATCH(dtype, CALL)                  \
   ((dtype) == OBB_F32 ? [&] { using T = float; return CALL; }() : (dtype) == OBB_BF16 ? [&] { using T = __bf16; return CALL; }() \
                                                                                 : [&] { using T = _Float16; return CALL; }())
@@ -279,7 +285,7 @@ extern "C" int obb_linear_forward(const void *x, int64_t ldx, const void *w, int
   if (m == 0 || n == 0) return OBB_OK;
   if (!y || (k > 0 && (!x || !w))) return set_err(OBB_EINVAL, "obb_linear_forward: null pointer");
   if ((m > 1 && ldx < k) || ldw < k || (res && ldr != 0 && ldr < n)) return set_err(OBB_EINVAL, "obb_linear_forward: row pitch below the row length");
-  if (ws_bytes < obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_FORWARD)) return set_err(OBB_EWORKSPACE, "obb_linear_forward: workspace too small");
+  if (int rc = check_workspace("obb_linear_forward", ws, ws_bytes, obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_FORWARD))) return rc;
   return OBB_LIN_DISPATCH(dtype, ([&] {
     Gemm<T> g = {(const T *)x, (const T *)w, ldx, ldw, m, n, k, (const T *)bias, (const T *)res, ldr, (T *)y, z, act};
     return gemm<T, false, false>(g, (float *)ws, (hipStream_t)stream);
@@ -295,8 +301,8 @@ extern "C" int obb_linear_act_backward(const void *dy, const void *y, const floa
   if (m > 0 && ((act == OBB_ACT_RELU && !y) || (act > OBB_ACT_RELU && !z)))
     return set_err(OBB_EINVAL, "obb_linear_act_backward: relu needs y, gelu and silu need z");
   if (!dz && !dbias) return set_err(OBB_EINVAL, "obb_linear_act_backward: nothing to write");
-  if (dbias && (!ws || ws_bytes < obb_linear_workspace_bytes(m, n, 0, dtype, OBB_LINEAR_ACT_BACKWARD)))
-    return set_err(OBB_EWORKSPACE, "obb_linear_act_backward: workspace too small");
+  if (dbias)
+    if (int rc = check_workspace("obb_linear_act_backward", ws, ws_bytes, obb_linear_workspace_bytes(m, n, 0, dtype, OBB_LINEAR_ACT_BACKWARD))) return rc;
   return OBB_LIN_DISPATCH(dtype, (act_backward<T>(dy, y, z, m, n, act, dz, dbias, ws, (hipStream_t)stream)));
 }
 
@@ -306,8 +312,7 @@ extern "C" int obb_linear_backward_input(const void *dz, const void *w, int64_t 
   if (m == 0 || k == 0) return OBB_OK;
   if (!dx || (n > 0 && (!dz || !w))) return set_err(OBB_EINVAL, "obb_linear_backward_input: null pointer");
   if (ldw < k) return set_err(OBB_EINVAL, "obb_linear_backward_input: row pitch below the row length");
-  if (ws_bytes < obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_BACKWARD_INPUT))
-    return set_err(OBB_EWORKSPACE, "obb_linear_backward_input: workspace too small");
+  if (int rc = check_workspace("obb_linear_backward_input", ws, ws_bytes, obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_BACKWARD_INPUT))) return rc;
   return OBB_LIN_DISPATCH(dtype, (plain_gemm<T, false, true>(dz, n, w, ldw, m, k, n, dx, ws, (hipStream_t)stream)));
 }
 
@@ -317,7 +322,6 @@ extern "C" int obb_linear_backward_weight(const void *dz, const void *x, int64_t
   if (n == 0 || k == 0) return OBB_OK;
   if (!dw || (m > 0 && (!dz || !x))) return set_err(OBB_EINVAL, "obb_linear_backward_weight: null pointer");
   if (m > 1 && ldx < k) return set_err(OBB_EINVAL, "obb_linear_backward_weight: row pitch below the row length");
-  if (ws_bytes < obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_BACKWARD_WEIGHT))
-    return set_err(OBB_EWORKSPACE, "obb_linear_backward_weight: workspace too small");
+  if (int rc = check_workspace("obb_linear_backward_weight", ws, ws_bytes, obb_linear_workspace_bytes(m, n, k, dtype, OBB_LINEAR_BACKWARD_WEIGHT))) return rc;
   return OBB_LIN_DISPATCH(dtype, (plain_gemm<T, true, true>(dz, n, x, ldx, n, k, m, dw, ws, (hipStream_t)stream)));
 }

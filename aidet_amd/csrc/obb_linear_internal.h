@@ -50,6 +50,7 @@ __device__ __forceinline__ float act_value(float z, int act) {
 // denormal), z for gelu and silu.
 __device__ __forceinline__ float act_slope(float v, int act) {
   if (act == OBB_ACT_RELU) return v != v ? v : (v > 0.f ? 1.f : 0.f);
+  if (act > OBB_ACT_RELU && fabsf(v) > 104.f) return v > 0.f ? 1.f : 0.f;     // (infinities too: no inf * 0)
   if (act == OBB_ACT_GELU)
     return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * expf(-0.5f * v * v) * 0.39894228040143268f;
   if (act == OBB_ACT_SILU) {
@@ -185,7 +186,7 @@ __device__ __forceinline__ void tile_out(const Gemm<T> &g, const f32x4 (&acc)[FM
     return;
   }
   constexpr uintptr_t A = 4 * sizeof(T) - 1;
-  const bool whole = (g.n & 3) == 0 && ((uintptr_t)g.y & A) == 0 && ((uintptr_t)g.res & A) == 0 && (g.ldr & 3) == 0;
+  const bool whole = (g.n & 3) == 0 && ((uintptr_t)g.y & A) == 0 && ((uintptr_t)g.res & A) == 0 && ((uintptr_t)g.z & 15) == 0 && (g.ldr & 3) == 0;
   if (whole) {
     // four columns of a row as one access: the fragments of a row's 64 columns leave one after the other and L2 joins them
     f32x4 bias[FN] = {};

@@ -1,14 +1,19 @@
 // obb_linear_mfma.hip -- the tiled product of 16-bit operands: C (M, N) = sum_k A(m, k) B(n, k), epilogue of the fused
 // linear layer, either operand stored with its contraction innermost ("rows") or outermost ("columns").
 //
-// A workgroup owns a BM x BN tile and walks K in steps of 32 through LDS slots, three per operand (two for the second where LDS ends): memory -> LDS without registers
-// in between (buffer loads that write LDS), LDS -> fragments one step ahead, fragments -> matrix instructions.  One barrier a
-// step: behind it the slot whose fragments everybody has taken is filled again, four steps before it is needed.
-// What bounds it: the matrix pipe, once the loads' latency is covered.  With two slots of 64 k (one in flight at a time) the
-// loads alone took 815 of 908 us at 8192 x 4096 x 16384; it is their latency, not their bytes (L2 hits 79 %).
+// A workgroup owns a BM x BN tile and walks K in slabs of 64: memory -> LDS without registers in between (buffer loads that
+// write LDS; three slots for the first operand, two or three for the second), LDS -> fragments half a slab ahead, fragments ->
+// matrix instructions.  One barrier a slab, in its middle: when everybody has the second half's fragments, the slab's slots
+// are free for loads that are due a slab later.  A wave issues in order, so loads, LDS reads and matrix instructions are dealt
+// evenly by hand: eight loads in a row held the matrix pipe back (4096 x 16384 x 4096: 427 us, dealt 402).
+// What bounds it: at 8192 x 4096 x 16384 (895 us with relu = 1228 TFLOP/s) the matrix pipe is busy 64 % at 1.9 GHz; without the
+// loads 727 us, without the matrix instructions 680: the slabs' latency behind L2 (79 % hits) is not all covered, and
+// every round of tiles begins and ends with an idle matrix pipe (about 10 us of 110).  Tried: slots of 32 k, five deep (rows
+// of 64 bytes double the L2 requests: 957 us), 32 x 32 instructions (1010), four waves of 128 x 128 (1000), raised priority
+// around the matrix instructions (930).
 //
-// LDS layout.  "rows": two rows of 32 k (64 bytes) make a line of eight 16-byte chunks; chunk c of row r sits at
-// ((r & 1) 4 + c) ^ (r >> 1 & 7) of line r / 2: the 16 rows of a fragment, read 16 bytes a lane, spread over all banks.
+// LDS layout.  "rows": [row][64 k], 128 bytes a row in eight 16-byte chunks, chunk c of row r kept at c ^ (r & 7): the 16
+// rows of a fragment, read 16 bytes a lane, spread over all banks (no conflicts counted).
 // "columns": [k][rows], chunk c of row k kept at c ^ turn(k), read with the transposing LDS load (a group of 16 lanes reads
 // 4 k x 16 rows and each lane gets 4 k of one row): the eight rows of k that 32 lanes read at once fall on different banks, and
 // pairs of chunks stay together.  The loads write LDS in lane order, so the exchange is made in the address a lane reads.
@@ -23,7 +28,6 @@ namespace obb {
 namespace lin {
 
 constexpr int BK = 64;
-
 
 template <typename T> struct Vec8;
 template <> struct Vec8<__bf16> { typedef bf16x8 v; };
@@ -53,16 +57,16 @@ constexpr uint32_t OUTSIDE = 0x80000000u;   // beyond every descriptor's size
 // the exchange of chunks in row k of a "columns" slot
 template <int R> __device__ __forceinline__ int turn(int k) { return (2 * ((k & 3) | (k >> 1 & 4))) & (R / 8 - 1); }
 
-// One operand's slot of `R` rows x 32 k: `R` / 16 wave loads, dealt over the workgroup's waves.
+// One operand's slot of `R` rows x 64 k: `R` / 8 wave loads, dealt over the workgroup's waves.
 template <typename T, int R, int WAVES, bool TR>
 struct Slab {
   static constexpr int LOADS = R / 8 / WAVES;
   static constexpr int BYTES = R * BK * 2;
   static_assert(LOADS * 8 * WAVES == R, "");
-  uint32_t off[LOADS];   // byte offset within the step, or OUTSIDE
+  uint32_t off[LOADS];   // byte offset within the slab, or OUTSIDE
   int kof[LOADS];        // first k of the lane's chunk
-  const char *base;      // of step 0
-  int64_t step;          // bytes from step to step
+  const char *base;      // of slab 0
+  int64_t step;          // bytes from slab to slab
 
   __device__ __forceinline__ void init(const T *p, int64_t ld, int64_t r0, int64_t rows, int64_t k0, int wave, int lane) {
     base = (const char *)p + (TR ? (k0 * ld + r0) * 2 : (r0 * ld + k0) * 2);

@@ -1,13 +1,16 @@
 // obb_linear_split.hip -- the tiled product of fp32 operands on the bf16 matrix instructions.
 //
 // An fp32 number is the exact sum of three bf16 numbers (24 = 8 + 8 + 8 significant bits):
-//   h = x cut to 8 bits,  m = x - h rounded to 8 bits,  l = the rest, exact    (|m| <= 2^-7 |h|, |l| <= 2^-8 |m|)
-// and x y = hh + (hm + mh) + (hl + lh + mm) + (ml + lm + ll); the last three are below 2^-22 of hh' product times 2^-2 each, of
-// either sign, and left out: at most 2^-23 |x y|, a rounding of the fp32 product itself is 2^-24.  Six bf16 products of exact
-// terms, added in fp32 by the matrix unit, cost 6 / 16 of what the fp32 matrix instruction takes.  (h is cut, not rounded, so
-// that no part overflows; bf16 has fp32's exponents, and the matrix unit keeps denormals, so parts vanish only below 2^-133.)
-// An infinite operand would give inf - inf in its own parts: a workgroup that finds NaNs in its sums computes those again with
-// the fp32 matrix instruction, whose infinities and NaNs are IEEE's.
+//   h = x rounded to 8 bits,  m = x - h rounded to 8 bits,  l = the rest, exact       (|m| <= 2^-8 |h|, |l| <= 2^-8 |m|)
+// and x y = hh + (hm + mh) + (hl + lh + mm) + (ml + lm + ll).  The last three are left out: of either sign and at most
+// 2^-23 |x y| together, where one rounding of the fp32 product is 2^-24.  Six bf16 products, exact and added in fp32 by the
+// matrix unit, take 6 / 16 of the fp32 matrix instruction's time.  (bf16 has fp32's exponents and the matrix unit keeps
+// denormals: parts vanish only below 2^-133.)
+// Where a part overflows -- x infinite, or within 2^-9 of the largest number -- x - h is not finite and the sum is a NaN: a
+// workgroup that finds NaNs in its sums computes those again with the fp32 matrix instruction, whose infinities and NaNs are
+// IEEE's.
+// What bounds it: 4096^3 615 us = 224 TFLOP/s (the fp32 matrix instruction's library product: 154), matrix pipe busy 66 % at
+// 1.96 GHz; the rest is splitting (two vector instructions a matrix instruction) and the two barriers of a step.
 #include "obb_linear_internal.h"
 
 namespace obb {
@@ -33,9 +36,8 @@ __device__ __forceinline__ Parts split8(const float (&x)[8]) {
   Parts p;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
-    p.h[i] = __builtin_amdgcn_perm(b, a, 0x07060302u);    // the upper halves
-    const float ra = x[2 * i] - __uint_as_float(a & 0xffff0000u), rb = x[2 * i + 1] - __uint_as_float(b & 0xffff0000u);
+    p.h[i] = pack(x[2 * i], x[2 * i + 1]);
+    const float ra = x[2 * i] - __uint_as_float(p.h[i] << 16), rb = x[2 * i + 1] - __uint_as_float(p.h[i] & 0xffff0000u);
     p.m[i] = pack(ra, rb);
     p.l[i] = pack(ra - __uint_as_float(p.m[i] << 16), rb - __uint_as_float(p.m[i] & 0xffff0000u));
   }

@@ -56,6 +56,7 @@ variable_list once(variable_list grads) {
       g.set_requires_grad(true);
       given.push_back(g);
     }
+  if (given.empty()) return grads;
   auto error = std::make_shared<torch::autograd::DelayedError>("trying to differentiate twice a function that is differentiable once", (int64_t)given.size());
   variable_list out = (*error)(std::move(given));
   size_t i = 0;
@@ -120,13 +121,17 @@ struct FusedLinear : public torch::autograd::Function<FusedLinear> {
     at::Tensor y, z;
     std::tie(y, z) = linear_forward(x, w, bias, res, (int)act, smooth);
     ctx->saved_data["act"] = act;
-    ctx->saved_data["need"] = (int64_t)((x.requires_grad() ? 1 : 0) | (w.requires_grad() ? 2 : 0) | (bias && bias->requires_grad() ? 4 : 0) |
-                                        (res && res->requires_grad() ? 8 : 0));
+    ctx->saved_data["bias"] = bias.has_value();
+    ctx->saved_data["residual"] = res.has_value();
     ctx->save_for_backward({x, w, smooth ? z : act == OBB_ACT_RELU ? y : at::Tensor()});
     return y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    const int64_t act = ctx->saved_data["act"].toInt(), need = ctx->saved_data["need"].toInt();
+    const int64_t act = ctx->saved_data["act"].toInt();
+    const bool bias = ctx->saved_data["bias"].toBool(), residual = ctx->saved_data["residual"].toBool();
+    // (a node's inputs are counted without those that are not there)
+    const int need = (ctx->needs_input_grad(0) ? 1 : 0) | (ctx->needs_input_grad(1) ? 2 : 0) | (bias && ctx->needs_input_grad(2) ? 4 : 0) |
+                     (residual && ctx->needs_input_grad(bias ? 3 : 2) ? 8 : 0);
     const auto saved = ctx->get_saved_variables();
     variable_list out(5);
     {

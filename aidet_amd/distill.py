@@ -20,7 +20,7 @@ def topk_distill_loss(logits, teacher_values, teacher_indices, temperature=1.0, 
         teacher_values (Tensor): (..., k) teacher logits, a constant (no gradient); k <= 1024
         teacher_indices (Tensor): (..., k) int64 / int32 classes; an index outside [0, C) marks an absent entry, an index
             that comes twice counts twice
-        temperature (float): T > 0
+        temperature (float): T, from 1e-6 to 1e6
         weight (Tensor, optional): (...) weight per row, a constant
         reduction (str): 'none' | 'mean' | 'sum'
         avg_factor (float, optional): with 'mean', the sum is divided by it instead of by the number of rows
@@ -33,8 +33,8 @@ def topk_distill_loss(logits, teacher_values, teacher_indices, temperature=1.0, 
     NotImplementedError: a tensor that is not on a HIP device.
     """
     temperature = float(temperature)
-    if not 0. < temperature < 3e38:
-        raise ValueError('temperature must be positive and finite, but got {}'.format(temperature))
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError('temperature must lie in [1e-6, 1e6], but got {}'.format(temperature))
     if reduction not in ('none', 'mean', 'sum'):
         raise ValueError("reduction must be 'none', 'mean' or 'sum', but got {!r}".format(reduction))
     scale = -1. if reduction == 'none' else 1.

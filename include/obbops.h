@@ -679,7 +679,7 @@ OBB_API int obb_linear_backward_weight(const void *dz_dev, const void *x_dev, in
  * their logits hold; an index that comes twice counts twice.  p_j = 0 adds nothing (also where q is 0); logits of -inf have
  * q = 0.  No gradient reaches the teacher.
  *   dtype / vtype     OBB_F32 / OBB_BF16 / OBB_F16 of logits (and dlogits) / of the teacher's values; index_bytes 4 or 8
- *   weight_dev        (rows) fp32, or NULL = 1;   k <= OBB_DISTILL_MAX_K
+ *   weight_dev        (rows) fp32, or NULL = 1;   k <= OBB_DISTILL_MAX_K;   temperature T in [1e-6, 1e6]
  *   row_loss_dev      (rows) fp32;   stats_dev (rows, 2) fp32, what the backward needs (NULL: no backward follows)
  *   loss_dev          one fp32, or NULL: only the rows' losses are wanted
  *   workspace_dev     obb_topk_distill_workspace_bytes(rows, classes) bytes (16-byte aligned; 0 bytes: may be NULL)

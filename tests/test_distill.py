@@ -105,6 +105,8 @@ def _idx(*shape, dtype=torch.int64):
     ((_fake(3, 4), _fake(3, 1025), _idx(3, 1025)), {}, ValueError),
     ((_fake(3, 4), _fake(3, 2), _idx(3, 2)), dict(temperature=0.), ValueError),
     ((_fake(3, 4), _fake(3, 2), _idx(3, 2)), dict(temperature=float('nan')), ValueError),
+    ((_fake(3, 4), _fake(3, 2), _idx(3, 2)), dict(temperature=1e-7), ValueError),
+    ((_fake(3, 4), _fake(3, 2), _idx(3, 2)), dict(temperature=float('inf')), ValueError),
     ((_fake(3, 4), _fake(3, 2), _idx(3, 2)), dict(weight=_fake(2)), ValueError),
     ((_fake(3, 4), _fake(3, 2), _idx(3, 2)), dict(weight=_idx(3)), ValueError),
     ((_fake(3, 4), _fake(3, 2), _idx(3, 2)), dict(weight=_fake(3).requires_grad_(True)), ValueError),

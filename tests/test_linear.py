@@ -261,6 +261,43 @@ def test_fp32_keeps_its_range(m, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('m, n', [(3, 40), (140, 200)])
+def test_fp32_numbers_at_the_ends_of_the_range(m, n):
+    """one factor a power of two, one term a sum: the products are exact, also of the largest and of denormal numbers"""
+    from aidet_amd import fused_linear
+    g = torch.Generator(device=DEV).manual_seed(18)
+    x = torch.zeros(m, 64, device=DEV)
+    top = torch.finfo(torch.float32).max
+    x[:, 0] = top * (1 - torch.rand(m, generator=g, device=DEV) * 2.0 ** -9)
+    x[0, 0], x[1, 0] = top, -top
+    w = torch.zeros(n, 64, device=DEV)
+    w[:, 0] = 1.
+    w[::2, 0] = 0.5
+    assert torch.equal(fused_linear(x, w), (x[:, :1].double() * w[:, 0].double()).float())
+    assert torch.equal(fused_linear(x[:, :1], w[:, :1]), fused_linear(x, w))
+    x[:, 0] = (torch.randint(1, 1 << 20, (m, ), generator=g, device=DEV).double() * 2.0 ** -149).float()
+    want = x[:, :1].double() * w[:, 0].double()
+    assert float((fused_linear(x, w).double() - want).abs().max()) <= 2.0 ** -133       # (parts below bf16's last bit vanish)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_activations_at_infinity(dtype):
+    """gelu and silu of +-inf are inf and 0, their slopes 1 and 0; NaN stays NaN"""
+    from aidet_amd import fused_linear
+    inf = float('inf')
+    x = torch.tensor([[inf], [-inf], [float('nan')], [200.], [-200.], [0.]], device=DEV, dtype=dtype).expand(6, 1).contiguous()
+    w = torch.ones(9, 1, device=DEV, dtype=dtype)
+    for act in ('gelu', 'silu', 'relu'):
+        r = torch.zeros(6, 9, device=DEV, dtype=dtype, requires_grad=True)
+        y = fused_linear(x, w, None, r, act)
+        assert torch.equal(y[[0, 1, 3, 4, 5]].abs(), torch.tensor([inf, 0., 200., 0., 0.], device=DEV, dtype=dtype)[:, None].expand(5, 9))
+        assert bool(y[2].isnan().all())
+        dr, = torch.autograd.grad(y, r, torch.ones_like(y))
+        assert torch.equal(dr[[0, 1, 3, 4]], torch.tensor([1., 0., 1., 0.], device=DEV, dtype=dtype)[:, None].expand(4, 9))
+
+
+@pytest.mark.gpu
 def test_pitches_past_32_bits():
     """rows 2^31 and more elements apart"""
     from aidet_amd import fused_linear
@@ -380,6 +417,18 @@ def test_gradients_only_where_wanted_and_broadcast(dtype):
     assert torch.equal(dr, torch.full_like(dr, 50.))
     v, s = product64(torch.ones(40, 50, device=DEV), x)
     assert bool(((dw.double() - v).abs() <= summed(s, 50, v.abs()) + half_step(dtype) * v.abs()).all())
+    # each gradient alone, with and without a bias before the residual
+    for with_bias in (True, False):
+        xs = x.detach().requires_grad_(True)
+        bs = b.detach().requires_grad_(True) if with_bias else None
+        rs = torch.randn(50, 40, device=DEV).to(dtype).requires_grad_(True)
+        y = fused_linear(xs, w, bs, rs, 'silu')
+        up = torch.randn(50, 40, device=DEV).to(dtype)
+        leaves = [xs, w] + ([bs] if with_bias else []) + [rs]
+        every = torch.autograd.grad(y, leaves, up, retain_graph=True)
+        for leaf, want in zip(leaves, every):
+            alone, = torch.autograd.grad(y, leaf, up, retain_graph=True)
+            assert torch.equal(alone, want)
     # the same weight twice in one graph: the gradients add
     x.requires_grad_(True)
     sq = (torch.randn(64, 64, device=DEV) / 8).to(dtype).requires_grad_(True)
