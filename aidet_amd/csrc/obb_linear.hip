@@ -111,8 +111,7 @@ int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
 }
 
 // ---- dz = dy act'(z) and db = sum_m dz: one pass over dy, column sums in two fixed steps (no atomics: the same bits
-// every run).  Block (x, y): 64 columns, rows y, y + chunks, ... of CS_ROWS; 16-byte accesses where the rows are aligned, four rows
-// under way a thread; partial sums [chunk][n] in the workspace.
+// every run).  Block (x, y): 64 columns, rows y, y + chunks, ... of a few dozen; 16-byte accesses, four rows under way a thread; partial sums [chunk][n] in the workspace.
 constexpr int CS_COLS = 64;
 template <typename T> constexpr int cs_rows() { return 256 / (CS_COLS * (int)sizeof(T) / 16) * 4; }     // rows a block takes at once
 static int colsum_chunks(int64_t m, int64_t n, int dtype) {
@@ -123,13 +122,13 @@ static int colsum_chunks(int64_t m, int64_t n, int dtype) {
 
 template <typename T>
 __global__ __launch_bounds__(256) void act_backward_kernel(const T *dy, const T *y, const float *z, int64_t m, int64_t n, int act,
-                                                           T *dz, float *partial, bool aligned) {
+                                                           T *dz, float *partial) {
   constexpr int W = 16 / sizeof(T), G = CS_COLS / W, RP = 256 / G;      // columns a thread, threads a row, rows a pass
-  typedef T tw __attribute__((ext_vector_type(W)));
+  typedef typename Loose<T, W>::v tw;
   __shared__ float sums[RP][CS_COLS + 1];
   const int c = threadIdx.x % G, r = threadIdx.x / G;
   const int64_t col = (int64_t)blockIdx.x * CS_COLS + c * W;
-  const bool whole = aligned && col + W <= n;
+  const bool whole = col + W <= n;
   float sum[W] = {};
   for (int64_t r0 = (int64_t)blockIdx.y * (4 * RP); r0 < m; r0 += (int64_t)gridDim.y * (4 * RP)) {
     float d[4][W], v[4][W];
@@ -149,7 +148,7 @@ __global__ __launch_bounds__(256) void act_backward_kernel(const T *dy, const T 
         } else if (act != OBB_ACT_NONE) {
 #pragma unroll
           for (int e = 0; e < W; e += 4) {
-            const f32x4 u = *(const f32x4 *)(z + at + e);
+            const f32x4 u = *(const Loose<float, 4>::v *)(z + at + e);
             v[q][e] = u[0], v[q][e + 1] = u[1], v[q][e + 2] = u[2], v[q][e + 3] = u[3];
           }
         }
@@ -228,9 +227,8 @@ static int act_backward(const void *dy, const void *y, const float *z, int64_t m
                         void *ws, hipStream_t stream) {
   const int chunks = colsum_chunks(m, n, sizeof(T) == 4 ? OBB_F32 : OBB_BF16);
   float *partial = db ? (float *)ws : nullptr;
-  const bool aligned = n * sizeof(T) % 16 == 0 && (((uintptr_t)dy | (uintptr_t)y | (uintptr_t)z | (uintptr_t)dz) & 15) == 0;
   act_backward_kernel<T><<<dim3((unsigned)((n + CS_COLS - 1) / CS_COLS), chunks), 256, 0, stream>>>(
-      (const T *)dy, (const T *)y, z, m, n, act, (T *)dz, partial, aligned);
+      (const T *)dy, (const T *)y, z, m, n, act, (T *)dz, partial);
   OBB_LAUNCH_CHECK();
   if (db) {
     colsum_join_kernel<T><<<(unsigned)((n + 63) / 64), 256, 0, stream>>>(partial, chunks, n, (T *)db);

@@ -74,24 +74,14 @@ struct Gemm {
   int act;
 };
 
-template <typename T, int ACT = -1>
-__device__ __forceinline__ void epilogue(const Gemm<T> &g, int64_t m, int64_t n, float acc) {
-  if (g.bias) acc += to_f32(g.bias[n]);
-  if (g.res) acc += to_f32(g.res[m * g.ldr + n]);
-  const int64_t at = m * g.n + n;
-  if (g.z) g.z[at] = acc;
-  g.y[at] = from_f32<T>(act_value(acc, ACT < 0 ? g.act : ACT));
-}
+// Vectors at any element's address: the memory unit takes them (an access more where they cross a line), so rows need not be
+// aligned for wide accesses, only inside.
+template <typename T, int W> struct Loose { typedef T v __attribute__((ext_vector_type(W), aligned(sizeof(T)))); };
 
-// What eight consecutive columns n .. n + 7 need of the epilogue whatever their row: the bias, and whether 16-byte accesses
-// are possible (all eight inside, rows and pointers aligned).
+// What eight consecutive columns n .. n + 7 need of the epilogue whatever their row
 struct Columns {
   float bias[8];
-  bool whole, whole_res;
   template <typename T> __device__ __forceinline__ void load(const Gemm<T> &g, int64_t n) {
-    constexpr uintptr_t A = 15;
-    whole = n + 8 <= g.n && (g.n * sizeof(T) & A) == 0 && ((uintptr_t)g.y & A) == 0 && ((uintptr_t)g.z & A) == 0;
-    whole_res = whole && (g.ldr * sizeof(T) & A) == 0 && ((uintptr_t)g.res & A) == 0;
 #pragma unroll
     for (int e = 0; e < 8; e++) bias[e] = g.bias && n + e < g.n ? to_f32(g.bias[n + e]) : 0.f;
   }
@@ -99,26 +89,21 @@ struct Columns {
 
 template <typename T>
 __device__ __forceinline__ void epilogue8(const Gemm<T> &g, const Columns &c, int64_t m, int64_t n, f32x4 lo, f32x4 hi) {
-  typedef T t8 __attribute__((ext_vector_type(8)));
+  typedef typename Loose<T, 8>::v t8;
+  typedef typename Loose<float, 4>::v f4;
   float v[8];
 #pragma unroll
   for (int e = 0; e < 8; e++) v[e] = (e < 4 ? lo[e] : hi[e - 4]) + c.bias[e];
   const int64_t at = m * g.n + n;
-  if (c.whole) {
+  if (n + 8 <= g.n) {
     if (g.res) {
-      const T *r = g.res + m * g.ldr + n;
-      if (c.whole_res) {
-        const t8 q = *(const t8 *)r;
+      const t8 q = *(const t8 *)(g.res + m * g.ldr + n);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += to_f32((T)q[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] += to_f32(r[e]);
-      }
+      for (int e = 0; e < 8; e++) v[e] += to_f32((T)q[e]);
     }
     if (g.z) {
-      *(f32x4 *)(g.z + at) = f32x4{v[0], v[1], v[2], v[3]};
-      *(f32x4 *)(g.z + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+      *(f4 *)(g.z + at) = f4{v[0], v[1], v[2], v[3]};
+      *(f4 *)(g.z + at + 4) = f4{v[4], v[5], v[6], v[7]};
     }
     t8 out;
 #pragma unroll
@@ -136,21 +121,32 @@ __device__ __forceinline__ void epilogue8(const Gemm<T> &g, const Columns &c, in
   }
 }
 
-// four consecutive columns of a row, aligned (the caller has checked), bias added already
+// four consecutive columns of a row, bias added already
 template <typename T, int ACT>
 __device__ __forceinline__ void epilogue4(const Gemm<T> &g, int64_t m, int64_t n, f32x4 v) {
-  typedef T t4 __attribute__((ext_vector_type(4)));
-  if (g.res) {
-    const t4 q = *(const t4 *)(g.res + m * g.ldr + n);
-#pragma unroll
-    for (int e = 0; e < 4; e++) v[e] += to_f32((T)q[e]);
-  }
+  typedef typename Loose<T, 4>::v t4;
   const int64_t at = m * g.n + n;
-  if (g.z) *(f32x4 *)(g.z + at) = v;
-  t4 out;
+  if (n + 4 <= g.n) {
+    if (g.res) {
+      const t4 q = *(const t4 *)(g.res + m * g.ldr + n);
 #pragma unroll
-  for (int e = 0; e < 4; e++) out[e] = from_f32<T>(act_value(v[e], ACT));
-  *(t4 *)(g.y + at) = out;
+      for (int e = 0; e < 4; e++) v[e] += to_f32((T)q[e]);
+    }
+    if (g.z) *(typename Loose<float, 4>::v *)(g.z + at) = v;
+    t4 out;
+#pragma unroll
+    for (int e = 0; e < 4; e++) out[e] = from_f32<T>(act_value(v[e], ACT));
+    *(t4 *)(g.y + at) = out;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; e++)
+      if (n + e < g.n) {
+        float u = v[e];
+        if (g.res) u += to_f32(g.res[m * g.ldr + n + e]);
+        if (g.z) g.z[at + e] = u;
+        g.y[at + e] = from_f32<T>(act_value(u, ACT));
+      }
+  }
 }
 
 // the sums of one split, (m, n) fp32 in the workspace with rows of a multiple of eight columns (the padding holds whatever the
@@ -169,10 +165,9 @@ __device__ __forceinline__ void tile_of(uint32_t wg, uint32_t tiles_m, uint32_t 
 }
 
 // A wave's FM x FN fragments of sums go out.  They are C transposed: lane l holds, of fragment (i, j), row m0 + 16 i + l % 16
-// and the four columns n0 + 16 j + 4 (l / 16) ... + 3.  `part`: the split's sums instead of the epilogue; `mine`: 256 FN
-// floats of LDS of the wave's own (used where rows are not aligned).
+// and the four columns n0 + 16 j + 4 (l / 16) ... + 3.  `part`: the split's sums instead of the epilogue.
 template <typename T, int ACT, int FM, int FN>
-__device__ __forceinline__ void tile_out(const Gemm<T> &g, const f32x4 (&acc)[FM][FN], int64_t m0, int64_t n0, float *part, float *mine, int lane) {
+__device__ __forceinline__ void tile_out(const Gemm<T> &g, const f32x4 (&acc)[FM][FN], int64_t m0, int64_t n0, float *part, int lane) {
   const int64_t nw = n0 + 4 * (lane >> 4);      // of the lane's four columns in fragment j: + 16 j
   if (part) {
     const int64_t pitch = part_pitch(g.n);
@@ -185,38 +180,20 @@ __device__ __forceinline__ void tile_out(const Gemm<T> &g, const f32x4 (&acc)[FM
     }
     return;
   }
-  constexpr uintptr_t A = 4 * sizeof(T) - 1;
-  const bool whole = (g.n & 3) == 0 && ((uintptr_t)g.y & A) == 0 && ((uintptr_t)g.res & A) == 0 && ((uintptr_t)g.z & 15) == 0 && (g.ldr & 3) == 0;
-  if (whole) {
-    // four columns of a row as one access: the fragments of a row's 64 columns leave one after the other and L2 joins them
-    f32x4 bias[FN] = {};
-    if (g.bias)
+  // four columns of a row as one access: the fragments of a row's columns leave one after the other and L2 joins them
+  f32x4 bias[FN] = {};
+  if (g.bias)
 #pragma unroll
-      for (int j = 0; j < FN; j++)
+    for (int j = 0; j < FN; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (nw + 16 * j < g.n) bias[j][e] = to_f32(g.bias[nw + 16 * j + e]);
+      for (int e = 0; e < 4; e++)
+        if (nw + 16 * j + e < g.n) bias[j][e] = to_f32(g.bias[nw + 16 * j + e]);
 #pragma unroll
-    for (int i = 0; i < FM; i++) {
-      const int64_t m = m0 + 16 * i + (lane & 15);
+  for (int i = 0; i < FM; i++) {
+    const int64_t m = m0 + 16 * i + (lane & 15);
 #pragma unroll
-      for (int j = 0; j < FN; j++)
-        if (m < g.m && nw + 16 * j < g.n) epilogue4<T, ACT>(g, m, nw + 16 * j, acc[i][j] + bias[j]);
-    }
-  } else {
-    // element by element, in a loop, from LDS: a wave lays down 16 rows at a time
-#pragma unroll
-    for (int i = 0; i < FM; i++) {
-#pragma unroll
-      for (int j = 0; j < FN; j++) *(f32x4 *)(mine + (lane & 15) * FN * 16 + 16 * j + 4 * (lane >> 4)) = acc[i][j];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll 1
-      for (int e = lane; e < 16 * FN * 16; e += 64) {
-        const int64_t m = m0 + 16 * i + e / (FN * 16), n = n0 + e % (FN * 16);
-        if (m < g.m && n < g.n) epilogue<T, ACT>(g, m, n, mine[e]);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
+    for (int j = 0; j < FN; j++)
+      if (m < g.m && nw + 16 * j < g.n) epilogue4<T, ACT>(g, m, nw + 16 * j, acc[i][j] + bias[j]);
   }
 }
 

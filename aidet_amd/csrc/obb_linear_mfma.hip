@@ -189,7 +189,7 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mfma_kernel(Gemm<T> g, uint3
     }
   }
   wait_and_meet<0>();
-  tile_out<T, ACT, FM, FN>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, (float *)lds + wave * 256 * FN, lane);
+  tile_out<T, ACT, FM, FN>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, lane);
 }
 
 // ---- the same product where rows or edges are not aligned: through registers ----------------------------------------------
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256) void gemm_ragged_kernel(Gemm<T> g, uint32_t ti
     }
     __syncthreads();
   }
-  tile_out<T, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, (float *)lds + wave * 256 * F, lane);
+  tile_out<T, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, lane);
 }
 
 template <typename T, int B, bool TA, bool TB>

@@ -170,14 +170,14 @@ __global__ __launch_bounds__(256, B == 128 ? 2 : 3) void gemm_split_kernel(Gemm<
   // The small tile has registers left for the residual: it is requested here, beside the first operands, and its latency is
   // not the epilogue's.
   f32x4 before[F][F];
-  const bool early = B == 64 && splits == 1 && g.res && (g.n & 3) == 0 && (g.ldr & 3) == 0 && ((uintptr_t)g.res & 15) == 0;
+  const bool early = B == 64 && splits == 1 && g.res && (g.n & 3) == 0;
   if (early) {
 #pragma unroll
     for (int i = 0; i < F; i++)
 #pragma unroll
       for (int j = 0; j < F; j++) {
         const int64_t m = m0 + wm + 16 * i + (lane & 15), n = n0 + wn + 16 * j + 4 * (lane >> 4);
-        before[i][j] = m < g.m && n < g.n ? *(const f32x4 *)(g.res + m * g.ldr + n) : f32x4{};
+        before[i][j] = m < g.m && n < g.n ? *(const Loose<float, 4>::v *)(g.res + m * g.ldr + n) : f32x4{};
       }
   }
   if (steps > 0) {
@@ -282,7 +282,7 @@ __global__ __launch_bounds__(256, B == 128 ? 2 : 3) void gemm_split_kernel(Gemm<
       for (int j = 0; j < F; j++) acc[i][j] += before[i][j];
     g.res = nullptr;
   }
-  tile_out<float, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, (float *)lds + wave * 256 * F, lane);
+  tile_out<float, ACT, F, F>(g, acc, m0 + wm, n0 + wn, splits > 1 ? partial + (int64_t)split * g.m * part_pitch(g.n) : nullptr, lane);
 }
 
 template <int B, bool TA, bool TB>
