@@ -403,8 +403,11 @@ static int parts_of(int64_t rows, int64_t classes) {
   return (int)(want < have ? want : (have < 1 ? 1 : have));
 }
 
-// rows of up to 64 classes: 16 lanes of a wave (60000 x 60: 61 us, by a wave each 91; 60000 x 200 by 64 lanes 137, by a wave each 88)
+// Short rows by 16 lanes of a wave, longer ones by a wave each; the gradient's lanes take a row's entries one after the other.
+// 45231 rows, losses only: 111 classes 11 us, by a wave each 29; 500 classes 22, 31.  Loss and gradient: 200 classes, 4 entries
+// 58, 69; 250, 32 entries 70, 72; 250, 200 entries 278, 139; 500, 32 entries 108, 90.
 template <typename T, bool FORWARD> static bool short_rows(const Args &a, hipStream_t st) {
+  if (a.classes > (FORWARD ? 512 : a.k <= 64 ? 256 : 64)) return false;
 #define OBB_SHORT(G, E)                                                                                               \
   if (a.classes <= G * E) {                                                                                           \
     const unsigned blocks = (unsigned)((a.rows + 256 / G - 1) / (256 / G));                                           \
@@ -414,6 +417,9 @@ template <typename T, bool FORWARD> static bool short_rows(const Args &a, hipStr
   }
   OBB_SHORT(16, 1)
   OBB_SHORT(16, 4)
+  OBB_SHORT(16, 8)
+  OBB_SHORT(16, 16)
+  if constexpr (FORWARD) OBB_SHORT(16, 32)
 #undef OBB_SHORT
   return false;
 }
