@@ -405,9 +405,9 @@ static int parts_of(int64_t rows, int64_t classes) {
 
 // Short rows by 16 lanes of a wave, longer ones by a wave each; the gradient's lanes take a row's entries one after the other.
 // 45231 rows, losses only: 111 classes 11 us, by a wave each 29; 500 classes 22, 31.  Loss and gradient: 200 classes, 4 entries
-// 58, 69; 250, 32 entries 70, 72; 250, 200 entries 278, 139; 500, 32 entries 108, 90.
+// 58, 69; 250, 32 entries 70, 72; 250, 200 entries 278 (gradient alone by a wave 200), 139; 500, 32 entries 108, 90.
 template <typename T, bool FORWARD> static bool short_rows(const Args &a, hipStream_t st) {
-  if (a.classes > (FORWARD ? 512 : a.k <= 64 ? 256 : 64)) return false;
+  if (a.classes > (a.k > 64 ? 64 : FORWARD ? 512 : 256)) return false;
 #define OBB_SHORT(G, E)                                                                                               \
   if (a.classes <= G * E) {                                                                                           \
     const unsigned blocks = (unsigned)((a.rows + 256 / G - 1) / (256 / G));                                           \
