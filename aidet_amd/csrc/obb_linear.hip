@@ -167,7 +167,10 @@ __global__ __launch_bounds__(256) void act_backward_kernel(const T *dy, const T 
       if (row >= m) continue;
       if (act != OBB_ACT_NONE)
 #pragma unroll
-        for (int e = 0; e < W; e++) d[q][e] *= act_slope(v[q][e], act);
+        for (int e = 0; e < W; e++) {
+          if (act == OBB_ACT_RELU && v[q][e] <= 0.f) d[q][e] = 0.f;          // (also where dy is infinite or NaN)
+          else d[q][e] *= act_slope(v[q][e], act);
+        }
 #pragma unroll
       for (int e = 0; e < W; e++) sum[e] += d[q][e];
       if (dz && whole) {

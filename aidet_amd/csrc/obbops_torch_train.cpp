@@ -3,9 +3,12 @@
 // small head is bound by the host: a node in Python costs about 60 us a direction, these about 15.
 #include <torch/extension.h>
 
+#include <ATen/autocast_mode.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 
 #include <tuple>
 
@@ -63,6 +66,26 @@ variable_list once(variable_list grads) {
   for (auto &g : grads)
     if (g.defined()) g = out[i++];
   return grads;
+}
+
+// A leaf's gradient is added up on the stream where its accumulator was made, and the accumulator lives as long as any graph
+// of the leaf.  One of the default stream, which takes no part in a capture, would end a process that captures this pass: say so.
+void check_capture(void *stream) {
+  hipStreamCaptureStatus status;
+  if (hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  const auto node = torch::autograd::get_current_node();
+  const auto *exec = torch::autograd::get_current_graph_task_exec_info();
+  if (!node) return;
+  for (const auto &edge : node->next_edges()) {
+    auto *leaf = dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get());
+    if (!leaf) continue;
+    if (exec && !exec->empty()) {
+      const auto it = exec->find(leaf);
+      if (it == exec->end() || !it->second.should_execute()) continue;
+    }
+    const auto s = leaf->stream();
+    TORCH_CHECK(!s || s->id() != 0, "a backward pass is captured while a graph of the same leaves from the default stream is alive: free that graph's outputs before the capture");
+  }
 }
 
 // ---- fused linear ------------------------------------------------------------------------------------------------------
@@ -140,6 +163,7 @@ struct FusedLinear : public torch::autograd::Function<FusedLinear> {
       const int64_t n = w.size(0), k = w.size(1), m = leading(x);
       HIPGuardMasqueradingAsCUDA guard(x.device());
       void *stream = stream_of(x);
+      check_capture(stream);
       const int code = code_of(x.scalar_type());
       const at::Tensor dy = grads[0].contiguous();
       at::Tensor dz = dy;
@@ -173,11 +197,25 @@ struct FusedLinear : public torch::autograd::Function<FusedLinear> {
   }
 };
 
-at::Tensor fused_linear(const at::Tensor &x, const at::Tensor &w, const MaybeTensor &bias, const MaybeTensor &res, int64_t act) {
+at::Tensor linear(const at::Tensor &x, const at::Tensor &w, const MaybeTensor &bias, const MaybeTensor &res, int64_t act) {
   check_linear(x, w, bias, res, act);
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (bias && bias->requires_grad()) || (res && res->requires_grad())))
     return FusedLinear::apply(x, w, bias, res, act);
   return std::get<0>(linear_forward(x, w, bias, res, (int)act, false));
+}
+
+// under autocast the tensors are cast as those of torch's own linear layer are
+at::Tensor cast(const at::Tensor &t, at::ScalarType type) { return code_of(t.scalar_type()) >= 0 ? t.to(type) : t; }
+
+at::Tensor fused_linear(const at::Tensor &x, const at::Tensor &w, const MaybeTensor &bias, const MaybeTensor &res, int64_t act) {
+  if (x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA)) {
+    const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
+    c10::impl::ExcludeDispatchKeyGuard off(at::autocast::get_autocast_dispatch_key_from_device_type(at::kCUDA));
+    const at::Tensor cx = cast(x, type), cw = cast(w, type);
+    const MaybeTensor cb = bias ? MaybeTensor(cast(*bias, type)) : bias, cr = res ? MaybeTensor(cast(*res, type)) : res;
+    return linear(cx, cw, cb, cr, act);
+  }
+  return linear(x, w, bias, res, act);
 }
 
 // ---- distillation ------------------------------------------------------------------------------------------------------
@@ -236,6 +274,7 @@ struct TopkDistill : public torch::autograd::Function<TopkDistill> {
       const at::Tensor logits = saved[0], v = saved[1], i = saved[2], w = saved[3], stats = saved[4];
       const int64_t classes = logits.size(-1), rows = leading(logits);
       HIPGuardMasqueradingAsCUDA guard(logits.device());
+      check_capture(stream_of(logits));
       out[0] = at::empty(logits.sizes(), logits.options());
       if (out[0].numel() > 0) {
         const Rows s(logits, classes);

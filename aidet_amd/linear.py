@@ -29,7 +29,8 @@ def fused_linear(x, weight, bias=None, residual=None, act='none'):
             row is read in place
         act (str): 'none' | 'relu' | 'gelu' (exact) | 'silu'
 
-    All tensors are of one type (float32, bfloat16 or float16) and on one HIP device.  Differentiable once with respect to
+    All tensors are of one type (float32, bfloat16 or float16) and on one HIP device; under ``torch.autocast`` they are cast
+    to its type first, as those of ``torch.nn.functional.linear`` are.  Differentiable once with respect to
     every tensor.  TypeError: a type that is not served, or several; ValueError: shapes that do not fit, an unknown act;
     NotImplementedError: a tensor that is not on a HIP device.
     """

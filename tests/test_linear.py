@@ -170,6 +170,46 @@ def test_forward_sizes(m, k, n, dtype):
     check(x, w, None, None, 'none')
 
 
+@pytest.fixture
+def cut():
+    """``cut(tile, splits)`` forces how products are cut (where that is possible); restored afterwards"""
+    from aidet_amd import _lib
+
+    def force(tile, splits):
+        _lib.set_tuning(_lib.TUNE_LINEAR_TILE, tile)
+        _lib.set_tuning(_lib.TUNE_LINEAR_SPLITS, splits)
+    yield force
+    force(-1, -1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('tile', [256, 192, 128, 64])
+@pytest.mark.parametrize('splits', [1, 2, 8])
+def test_every_cut(tile, splits, dtype, cut):
+    """each tile and number of splits on sizes that end inside tiles, slabs and splits, forward and gradients, aligned and not"""
+    for m, k, n in ((300, 1096, 264), (300, 1001, 263), (40, 72, 24)):
+        x, w, b, r = make(m, k, n, dtype, True, True, seed=tile + splits)
+        dy = torch.randn(m, n, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV).to(dtype)
+        cut(tile, splits)
+        check(x, w, b, r, 'relu')
+        check_gradients(x, w, b, r, 'gelu', dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('m, k, n', [(4096, 128, 4352), (4000, 200, 4360), (2300, 192, 8200), (4104, 72, 4360)])
+def test_more_tiles_than_the_device_holds(m, k, n, cut):
+    """a workgroup takes several tiles one after the other, whole ones and ones that end inside, with few slabs each"""
+    cut(256, 1)
+    for dtype in TYPES[1:]:
+        x, w, b, r = make(m, k, n, dtype, True, True, seed=19)
+        check(x, w, b, r, 'silu')
+        check(x, w, None, None, 'none')
+        x, w, b, _ = make(n, k, m, dtype, True, False, seed=20)
+        dy = torch.randn(n, m, generator=torch.Generator(device=DEV).manual_seed(6), device=DEV).to(dtype)
+        check_gradients(x, w, b, None, 'gelu', dy)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', TYPES)
 @pytest.mark.parametrize('act', ['none', 'relu', 'gelu', 'silu'])
@@ -494,3 +534,86 @@ def test_captured_step_replays(dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, want)), i
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_infinite_gradients_of_units_that_are_off(dtype):
+    """relu: where y is 0 the gradient of y reaches nothing, whatever it holds"""
+    from aidet_amd import fused_linear
+    x, w, b, r = make(70, 200, 67, dtype, True, True, seed=23)
+    leaves = [t.requires_grad_(True) for t in (x.contiguous(), w, b, r)]
+    y = fused_linear(*leaves, act='relu')
+    dy = torch.randn(70, 67, generator=torch.Generator(device=DEV).manual_seed(7), device=DEV).to(dtype)
+    dy = torch.where(y > 0, dy, torch.zeros_like(dy))
+    odd = dy.clone()
+    for i, bad in enumerate((float('inf'), float('-inf'), float('nan'))):
+        odd[i::3] = torch.where(y[i::3] > 0, dy[i::3], torch.full_like(dy[i::3], bad))
+    want = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    got = torch.autograd.grad(y, leaves, odd)
+    assert all(bool(torch.isfinite(t).all()) and torch.equal(t, u) for t, u in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES[1:])
+def test_autocast_casts_as_a_linear_layer_does(dtype):
+    from aidet_amd import FusedLinear, fused_linear
+    x, w, b, r = make(33, 120, 50, torch.float32, True, True, seed=29)
+    layer = FusedLinear(120, 50, act='silu').to(DEV)
+    with torch.autocast('cuda', dtype=dtype):
+        y = fused_linear(x, w, b.to(torch.float16), r, 'silu')
+        z = layer(x.to(dtype), r)
+    assert y.dtype == dtype and z.dtype == dtype
+    assert torch.equal(y, fused_linear(x.to(dtype), w.to(dtype), b.to(torch.float16).to(dtype), r.to(dtype), 'silu'))
+    z.sum().backward()
+    assert layer.weight.grad.dtype == torch.float32 and bool(layer.weight.grad.abs().sum() > 0)
+    dy = torch.ones_like(z)
+    a, c = layer.weight.detach().to(dtype).requires_grad_(True), layer.bias.detach().to(dtype)
+    want, = torch.autograd.grad(fused_linear(x.to(dtype), a, c, r.to(dtype), 'silu'), a, dy)
+    assert torch.equal(layer.weight.grad, want.float())
+
+
+@pytest.mark.gpu
+def test_capture_beside_an_eager_graph_of_the_default_stream():
+    """a captured backward pass whose leaves' accumulators belong to the default stream is refused; afterwards it is served"""
+    from aidet_amd import fused_linear, topk_distill_loss
+    w = torch.randn(24, 40, device=DEV, requires_grad=True)
+    x = torch.randn(9, 40, device=DEV)
+    logits = torch.randn(9, 24, device=DEV, requires_grad=True)
+    values, indices = torch.randn(9, 4, device=DEV), torch.arange(36, device=DEV).reshape(9, 4) % 24
+
+    def linear():
+        return fused_linear(x, w, act='silu').square().sum()
+
+    def distill():
+        return topk_distill_loss(logits, values, indices)
+    for loss, leaf in ((linear, w), (distill, logits)):
+        kept = loss()
+        kept.backward()
+        want, leaf.grad = leaf.grad, None
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match='graph of the same leaves'):
+            with torch.cuda.graph(graph):
+                loss().backward()
+        torch.cuda.synchronize()
+        del kept
+        leaf.grad = None
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            kept = loss()                    # (alive during the capture, but not of the default stream)
+            kept.backward()
+        torch.cuda.current_stream().wait_stream(s)
+        leaf.grad = None
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            loss().backward()
+        for _ in range(3):
+            leaf.grad.zero_()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(leaf.grad, want)
+        del kept
+        leaf.grad = None
