@@ -111,16 +111,22 @@ int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
 }
 
 // ---- dz = dy act'(z) and db = sum_m dz: one pass over dy, column sums in two fixed steps (no atomics: the same bits
-// every run).  Block (x, y): 64 columns, rows y, y + chunks, ... of a few dozen; 16-byte accesses, four rows under way a thread; partial sums [chunk][n] in the workspace.
+// every run).  dz is rounded to the type once, as the two products take operands of the type; db sums what was not rounded.
+// Block (x, y): 64 columns, rows y, y + chunks, ... of a few dozen; 16-byte accesses, four rows under way a thread, or one where
+// four would leave the device short of workgroups (both kernels, us, four and one: 777 x 515 fp32 gelu 10.6, 7.6; 1024 x 1024
+// bf16 relu 7.7, 7.0); partial sums [chunk][n] in the workspace.  Larger ones are memory's: 8192 x 1024 fp32 silu 26.5 us = 3.8 TB/s.
 constexpr int CS_COLS = 64;
-template <typename T> constexpr int cs_rows() { return 256 / (CS_COLS * (int)sizeof(T) / 16) * 4; }     // rows a block takes at once
+static int colsum_depth(int64_t m, int64_t n, int dtype) {      // rows under way a thread
+  const int64_t rows = dtype == OBB_F32 ? 64 : 128;
+  return ((m + rows - 1) / rows) * ((n + CS_COLS - 1) / CS_COLS) < 512 ? 1 : 4;
+}
 static int colsum_chunks(int64_t m, int64_t n, int dtype) {
-  const int rows = dtype == OBB_F32 ? cs_rows<float>() : cs_rows<__bf16>();
+  const int rows = (dtype == OBB_F32 ? 16 : 32) * colsum_depth(m, n, dtype);      // rows a block takes at once
   const int64_t want = 4096 / ((n + CS_COLS - 1) / CS_COLS) + 1, have = (m + rows - 1) / rows;
   return (int)(want < have ? want : (have < 1 ? 1 : have));
 }
 
-template <typename T>
+template <typename T, int U>
 __global__ __launch_bounds__(256) void act_backward_kernel(const T *dy, const T *y, const float *z, int64_t m, int64_t n, int act,
                                                            T *dz, float *partial) {
   constexpr int W = 16 / sizeof(T), G = CS_COLS / W, RP = 256 / G;      // columns a thread, threads a row, rows a pass
@@ -130,10 +136,10 @@ __global__ __launch_bounds__(256) void act_backward_kernel(const T *dy, const T 
   const int64_t col = (int64_t)blockIdx.x * CS_COLS + c * W;
   const bool whole = col + W <= n;
   float sum[W] = {};
-  for (int64_t r0 = (int64_t)blockIdx.y * (4 * RP); r0 < m; r0 += (int64_t)gridDim.y * (4 * RP)) {
-    float d[4][W], v[4][W];
+  for (int64_t r0 = (int64_t)blockIdx.y * (U * RP); r0 < m; r0 += (int64_t)gridDim.y * (U * RP)) {
+    float d[U][W], v[U][W];
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
+    for (int q = 0; q < U; q++) {
       const int64_t row = r0 + q * RP + r, at = row * n + col;
 #pragma unroll
       for (int e = 0; e < W; e++) d[q][e] = 0.f, v[q][e] = 0.f;
@@ -162,7 +168,7 @@ __global__ __launch_bounds__(256) void act_backward_kernel(const T *dy, const T 
       }
     }
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
+    for (int q = 0; q < U; q++) {
       const int64_t row = r0 + q * RP + r, at = row * n + col;
       if (row >= m) continue;
       if (act != OBB_ACT_NONE)
@@ -230,8 +236,11 @@ static int act_backward(const void *dy, const void *y, const float *z, int64_t m
                         void *ws, hipStream_t stream) {
   const int chunks = colsum_chunks(m, n, sizeof(T) == 4 ? OBB_F32 : OBB_BF16);
   float *partial = db ? (float *)ws : nullptr;
-  act_backward_kernel<T><<<dim3((unsigned)((n + CS_COLS - 1) / CS_COLS), chunks), 256, 0, stream>>>(
-      (const T *)dy, (const T *)y, z, m, n, act, (T *)dz, partial);
+  const dim3 grid((unsigned)((n + CS_COLS - 1) / CS_COLS), chunks);
+  if (colsum_depth(m, n, sizeof(T) == 4 ? OBB_F32 : OBB_BF16) == 1)
+    act_backward_kernel<T, 1><<<grid, 256, 0, stream>>>((const T *)dy, (const T *)y, z, m, n, act, (T *)dz, partial);
+  else
+    act_backward_kernel<T, 4><<<grid, 256, 0, stream>>>((const T *)dy, (const T *)y, z, m, n, act, (T *)dz, partial);
   OBB_LAUNCH_CHECK();
   if (db) {
     colsum_join_kernel<T><<<(unsigned)((n + 63) / 64), 256, 0, stream>>>(partial, chunks, n, (T *)db);
