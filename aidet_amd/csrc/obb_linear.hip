@@ -86,6 +86,17 @@ Plan plan32(int64_t m, int64_t n, int64_t k) {
   return cheapest(cuts, 2, m, n, (k + 31) / 32);
 }
 
+// Few rows by one launch without splits: up to 32 rows whose K is one block a wave, where the tiled product would split K.
+// Measured, us, tiled and thin: 1 x 1024 x 1024 bf16 6.9, 3.7, fp32 8.5, 4.8; 24 x 2048 x 1024 bf16 8.8, 7.1; 24 x 1024 x 1024 fp32
+// 9.9, 8.2; 32 x 2048 x 4096 bf16 10.2, 8.0.  Beyond: K 24 x 4096 x 1024 bf16 9.5, 11.5; N 32 x 1024 x 16384 bf16 10.2, 14.1; rows at odd
+// 16-bit addresses 24 x 1001 x 1023 9.5, 11.7 (at even ones 9.6, 8.0); K not split 32 x 64 x 4096 4.1, 6.6.
+template <typename T> static bool thin(const Gemm<T> &g, const Plan &p) {
+  const int64_t force = tuning(OBB_TUNE_LINEAR_TILE, 0);
+  if (force || tuning(OBB_TUNE_LINEAR_SPLITS, 0)) return force == 16 && g.m <= 32;
+  const uintptr_t at = (uintptr_t)g.a | (uintptr_t)g.b | (uintptr_t)(g.lda * sizeof(T)) | (uintptr_t)(g.ldb * sizeof(T));
+  return g.m <= 32 && p.splits > 1 && g.k * (int64_t)sizeof(T) <= 4096 && g.n <= 4096 && at % 4 == 0;
+}
+
 static bool aligned16(const void *p, int64_t ld, int64_t extent) {
   return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && extent % 8 == 0;
 }
@@ -93,13 +104,14 @@ static bool aligned16(const void *p, int64_t ld, int64_t extent) {
 template <typename T, bool TA, bool TB>
 int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
   if (g.m == 0 || g.n == 0) return OBB_OK;
-  Plan p;
+  // (the same plan whatever the alignment: the workspace is sized without looking at pointers)
+  const Plan p = sizeof(T) == 4 ? plan32(g.m, g.n, g.k) : plan16(g.m, g.n, g.k);
   int rc;
+  if constexpr (!TA && !TB)
+    if (thin(g, p)) return gemm_thin<T>(g, stream);
   if constexpr (sizeof(T) == 4) {
-    p = plan32(g.m, g.n, g.k);
     rc = gemm_split<TA, TB>(g, p.tile, p.splits, ws, stream);
   } else {
-    p = plan16(g.m, g.n, g.k);      // (the same for both kernels: the workspace is sized without looking at pointers)
     // Direct loads need 16-byte chunks that end with the operand, and a slab that fits a buffer descriptor: 256 rows, or 64
     // where the contraction is outermost, below 2 GiB.  (4096^3 bf16: 105 us; 4095^3 through registers 250.)
     if (aligned16(g.a, g.lda, TA ? g.m : g.k) && aligned16(g.b, g.ldb, TB ? g.n : g.k) && g.lda < (1 << 22) - 256 && g.ldb < (1 << 22) - 256)

@@ -205,6 +205,9 @@ struct Plan { int tile, splits; };
 Plan plan16(int64_t m, int64_t n, int64_t k);
 Plan plan32(int64_t m, int64_t n, int64_t k);
 
+// at most 32 rows, both operands with their contraction innermost, any type and alignment (obb_linear_thin.hip)
+template <typename T> int gemm_thin(const Gemm<T> &g, hipStream_t stream);
+
 // fp32 operands, any alignment (obb_linear_split.hip)
 template <bool TA, bool TB> int gemm_split(const Gemm<float> &g, int tile, int splits, float *partial, hipStream_t stream);
 

@@ -727,7 +727,7 @@ OBB_API int obb_topk_distill_backward(const void *logits_dev, int64_t ld, int64_
 #define OBB_TUNE_NMS_RESOLVE_TAIL 19   /* resolve, bit 0: the last <= 4 edges per thread of a shard are retired from registers (1, default) or swept through memory (0); bit 1: the first sweep uses agent-scope loads like the others (measurement only); bit 2: the resolve reports itself stalled (test hook for OBB_ESTALLED) */
 #define OBB_TUNE_NMS_RESOLVE_PARTS 20   /* resolve of calls of >= 2^18 boxes: workgroups per edge shard (1 .. 16; never more than half of what the device keeps resident) */
 #define OBB_TUNE_NMS_RETAIN 21          /* 0: OBB_NMS_RETAIN is ignored (every call runs the frame launch): A/B measurements */
-#define OBB_TUNE_LINEAR_TILE 22         /* fused linear layer: tile of a product -- 256, 192 (= 256 x 128), 128 or 64 (fp32: 128 or 64; K <= 256 always 64; unaligned 16-bit operands: above 64 it is 128); < 0: by its cost */
+#define OBB_TUNE_LINEAR_TILE 22         /* fused linear layer: tile of a product -- 256, 192 (= 256 x 128), 128 or 64 (fp32: 128 or 64; K <= 256 always 64; unaligned 16-bit operands: above 64 it is 128), 16 = the forward product of up to 32 rows without splits; < 0: by its cost */
 #define OBB_TUNE_LINEAR_SPLITS 23       /* fused linear layer: splits of the contraction -- 1, 2, 4, 8 or 16, where it has two slabs a split; < 0: by their cost */
 #define OBB_TUNE_COUNT 24
 OBB_API int obb_set_tuning(int knob, int64_t value);

@@ -197,6 +197,44 @@ def test_every_cut(tile, splits, dtype, cut):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('forced', [False, True])
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m', [1, 2, 16, 17, 32, 33])
+def test_few_rows(m, dtype, forced, cut):
+    """rows up to 32 by one launch: K of one element, that ends inside a chunk, a block and a wave's share; odd N and pitches"""
+    from aidet_amd import fused_linear
+    if forced:
+        cut(16, 1)
+    for k, n, pad in ((1024, 1024, 0), (1, 17, 0), (3, 5, 0), (7, 40, 1), (8, 16, 0), (255, 31, 1), (256, 33, 0), (257, 100, 3), (1001, 1023, 3),
+                      (2047, 65, 1), (2048, 64, 0), (4100, 20, 4)):
+        x, w, b, r = make(m, k, n, dtype, True, True, seed=m + k, pad=pad)
+        check(x, w, b, r, 'gelu')
+        check(x, w, None, None, 'relu')
+    x, w, b, _ = make(m, 0, 50, dtype, True, False)
+    assert torch.equal(fused_linear(x, w, b, None, 'silu'), fused_linear(x.new_zeros(m, 1), w.new_zeros(50, 1), b, None, 'silu'))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+def test_few_rows_keep_infinities_and_nans_to_their_rows(dtype):
+    """a NaN or an infinity in a row of x or of w reaches that row or column alone, at the end of K too, and nothing outside K is read into a sum"""
+    from aidet_amd import fused_linear
+    k, n = 1000, 500
+    x, w, _, _ = make(5, k + 24, n, dtype, False, False, seed=3)
+    w = torch.cat([w[:, :k], torch.full((n, 24), float('nan'), device=DEV, dtype=dtype)], 1)[:, :k]     # (NaN behind every row)
+    x = torch.cat([x[:, :k], torch.full((5, 24), float('inf'), device=DEV, dtype=dtype)], 1)[:, :k]
+    want = check(x, w, None, None, 'none')
+    x2, w2 = x.clone(), w.clone()
+    x2[1, k - 1], x2[3, 0], w2[7, k - 1] = float('nan'), float('inf'), float('nan')
+    y = fused_linear(x2, w2)
+    assert bool(torch.isnan(y[1]).all()) and bool(torch.isnan(y[:, 7]).all())
+    assert not bool(torch.isfinite(y[3]).any())
+    keep = [0, 2, 4]
+    cols = [c for c in range(n) if c != 7]
+    assert torch.equal(y[keep][:, cols], want[keep][:, cols])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('m, k, n', [(4096, 128, 4352), (4000, 200, 4360), (2300, 192, 8200), (4104, 72, 4360)])
 def test_more_tiles_than_the_device_holds(m, k, n, cut):
     """a workgroup takes several tiles one after the other, whole ones and ones that end inside, with few slabs each"""
