@@ -339,6 +339,22 @@ def test_fp32_keeps_its_range(m, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('m', [3, 20])
+def test_few_fp32_rows_at_the_ends_of_the_range(m, cut):
+    """the product of few rows: one term a sum, a power of two the other factor: exact, the largest numbers and denormal ones too"""
+    from aidet_amd import fused_linear
+    cut(16, 1)
+    g = torch.Generator(device=DEV).manual_seed(31)
+    x, w = torch.zeros(m, 200, device=DEV), torch.zeros(40, 200, device=DEV)
+    w[:, 199] = 1.
+    w[::2, 199] = 0.5
+    x[:, 199] = torch.finfo(torch.float32).max
+    assert torch.equal(fused_linear(x, w), (x[:, 199:].double() * w[:, 199].double()).float())
+    x[:, 199] = (torch.randint(1, 1 << 20, (m, ), generator=g, device=DEV).double() * 2.0 ** -148).float()
+    assert torch.equal(fused_linear(x, w), (x[:, 199:].double() * w[:, 199].double()).float())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('m, n', [(3, 40), (140, 200)])
 def test_fp32_numbers_at_the_ends_of_the_range(m, n):
     """one factor a power of two, one term a sum: the products are exact, also of the largest and of denormal numbers"""
