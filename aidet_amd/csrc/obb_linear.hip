@@ -137,6 +137,7 @@ static int colsum_depth(int64_t m, int64_t n, int dtype) {      // rows under wa
   return ((m + rows - 1) / rows) * ((n + CS_COLS - 1) / CS_COLS) < 512 ? 1 : 4;
 }
 static int colsum_chunks(int64_t m, int64_t n, int dtype) {
+  if (n == 0) return 0;                                                           // (no column: no block, no sum)
   const int rows = (dtype == OBB_F32 ? 16 : 32) * colsum_depth(m, n, dtype);      // rows a block takes at once
   const int64_t want = 4096 / ((n + CS_COLS - 1) / CS_COLS) + 1, have = (m + rows - 1) / rows;
   return (int)(want < have ? want : (have < 1 ? 1 : have));

@@ -156,6 +156,17 @@ def test_c_abi_refusals_without_gpu():
     assert L.obb_linear_workspace_bytes(-1, 5, 4, 0, 0) == 0
 
 
+@pytest.mark.parametrize('op', range(4))
+@pytest.mark.parametrize('dtype', range(3))
+def test_workspaces_of_empty_sizes(op, dtype):
+    """each size zero in turn and together: a number of bytes that an empty output or an empty sum needs"""
+    from aidet_amd import _lib
+    size = _lib.lib().obb_linear_workspace_bytes
+    for m, n, k in ((0, 5, 8), (4, 0, 8), (4, 5, 0), (0, 0, 8), (0, 5, 0), (4, 0, 0), (0, 0, 0)):
+        have = size(m, n, k, dtype, op)
+        assert have == (256 if op == _lib.LINEAR_ACT_BACKWARD and n else 0), (m, n, k, have)
+
+
 # ---- values --------------------------------------------------------------------------------------------------------------
 SIZES = [(1, 1, 1), (1, 64, 64), (2, 7, 3), (17, 33, 65), (64, 64, 64), (1, 4096, 1000), (5, 1024, 16), (63, 129, 257), (128, 256, 128),
          (200, 1000, 80), (257, 512, 255), (1000, 72, 40), (300, 2056, 520), (4097, 24, 8), (33, 12544, 96)]
@@ -298,6 +309,24 @@ def test_empty_sizes(dtype):
     leaves = [t.requires_grad_(True) for t in (x, w, b)]
     dx, dw, db = torch.autograd.grad(fused_linear(*leaves, act='gelu').float().sum(), leaves)
     assert dx.shape == (0, 8) and not dw.any() and not db.any() and dw.shape == w.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('act', ['none', 'relu', 'gelu', 'silu'])
+@pytest.mark.parametrize('m, k, n', [(4, 8, 0), (4, 0, 5), (0, 8, 5), (0, 0, 5), (4, 0, 0), (0, 8, 0), (0, 0, 0)])
+def test_gradients_of_empty_sizes(m, k, n, act, dtype):
+    """every gradient has its tensor's shape: zeros where nothing is summed, with no terms in the product dz alone remains"""
+    x, w, b, r = make(m, k, n, dtype, True, True, seed=2)
+    dy = torch.ones(m, n, device=DEV, dtype=dtype)
+    dx, dw, db, dr = gradients(x, w, b, r, act, dy)
+    assert dx.shape == x.shape and dw.shape == w.shape and db.shape == b.shape and dr.shape == r.shape
+    assert not dx.any() if n == 0 else True
+    assert not dw.any()
+    if m and n:
+        check_gradients(x, w, b, r, act, dy)
+    else:
+        assert not db.any()
 
 
 @pytest.mark.gpu
