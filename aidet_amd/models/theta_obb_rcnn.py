@@ -81,7 +81,7 @@ class Bottleneck(nn.Module):
     @torch.no_grad()
     def fold(self, on=True):
         """`on`: conv1 + bn1 + ReLU and conv3 + bn3 + shortcut + ReLU run as one fused linear layer each on channels-last maps
-        in eval mode, with the weights of NOW (loading weights, or train(), ends it)."""
+        in eval mode, with the weights of NOW (loading weights, train(), or a pass with a norm in training mode ends it)."""
         for name in self._FOLDED:
             self.register_buffer(name, None, persistent=False)
         self.folded = bool(on)
@@ -102,6 +102,8 @@ class Bottleneck(nn.Module):
         super(Bottleneck, self)._load_from_state_dict(*args, **kwargs)
 
     def forward(self, x):
+        if self.folded and (self.training or self.bn1.training or self.bn3.training):
+            self.fold(False)        # (a norm in training mode goes by the batch, and moves the statistics that were folded)
         if self.folded and not torch.is_grad_enabled() and _channels_last(x):
             idt = x if self.downsample is None else self.downsample(x)
             out = F.relu(self.bn2(self.conv2(pointwise(x, self.w1, self.b1, act='relu'))), inplace=True)

@@ -43,6 +43,51 @@ def test_folding_is_dropped_with_the_weights_it_came_from():
     assert set(ThetaOBBRCNN(fused_linear=True).state_dict()) == keys
 
 
+@pytest.fixture
+def calls(monkeypatch):
+    """every map counts as channels-last on a device and `pointwise` is a plain convolution here: the list of its calls"""
+    import aidet_amd.models.theta_obb_rcnn as mod
+    made = []
+
+    def plain(x, weight, bias=None, residual=None, act='none'):
+        made.append(tuple(weight.shape))
+        y = torch.nn.functional.conv2d(x, weight[:, :, None, None], bias)
+        y = y if residual is None else y + residual
+        return y.relu() if act == 'relu' else y
+    monkeypatch.setattr(mod, '_channels_last', lambda x: True)
+    monkeypatch.setattr(mod, 'pointwise', plain)
+    return made
+
+
+def test_a_folded_bottleneck_in_training_mode_normalises_by_the_batch(calls):
+    """fold() after train(), and a norm alone in training mode: the batch's statistics, running ones updated; fold() of a
+    module in training mode serves once it is in eval mode, unless a pass has moved the statistics it was made of"""
+    import copy
+    from aidet_amd.models.theta_obb_rcnn import Bottleneck
+    torch.manual_seed(3)
+    for norms in (('bn1', 'bn2', 'bn3'), ('bn1', ), ('bn3', )):
+        plain = Bottleneck(16, 4).eval()
+        for name in norms:
+            getattr(plain, name).train()
+        if len(norms) == 3:
+            plain.train()
+        folded = copy.deepcopy(plain)
+        folded.fold()
+        assert folded.folded
+        x = torch.randn(2, 16, 5, 6)
+        with torch.no_grad():
+            want, got = plain(x), folded(x)
+            assert torch.equal(want, got) and not calls
+            assert all(torch.equal(u, v) for u, v in zip(plain.state_dict().values(), folded.state_dict().values()))
+            assert torch.equal(plain.eval()(x), folded.eval()(x)) and not calls    # (what was folded is not what it is now)
+            folded.train()
+            folded.fold()
+            folded.eval()
+            near = folded(x)
+        assert calls == [(4, 16), (16, 4)] and float((near - plain(x)).abs().max()) < 1e-5
+        calls.clear()
+
+
 @pytest.mark.gpu
 def test_heads_on_fused_layers():
     from aidet_amd.models.theta_obb_rcnn import SharedFCHead
