@@ -303,12 +303,22 @@ class ThetaOBBRCNN(nn.Module):
 
     def fold_pointwise(self, on=True):
         """Inference on channels-last maps: the bottlenecks' 1 x 1 convolutions (norm folded in, shortcut and ReLU in the
-        epilogue) and the FPN laterals run as fused linear layers.  Folds the weights of now: call it again after changing them."""
+        epilogue) and the FPN laterals run as fused linear layers.  Folds the weights of now: call it again after changing them
+        (loading weights and train() end it)."""
         for m in self.backbone.modules():
             if isinstance(m, Bottleneck):
                 m.fold(on)
         self.neck.fused_linear = bool(on)
         return self
+
+    def train(self, mode=True):
+        if mode:
+            self.neck.fused_linear = False       # (the bottlenecks see to themselves)
+        return super(ThetaOBBRCNN, self).train(mode)
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        self.neck.fused_linear = False
+        super(ThetaOBBRCNN, self)._load_from_state_dict(*args, **kwargs)
 
     # ---- timing hooks (bench): wall time per stage, device synchronised at the boundaries ----
     def _tick(self, name):
