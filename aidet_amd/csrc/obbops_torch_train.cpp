@@ -49,6 +49,12 @@ at::Tensor workspace(size_t bytes, const at::Tensor &like) {
 }
 void *ptr(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
+// Forward mode has no rule here: a dual tensor is refused, not read as its primal alone (which would be a derivative of 0).
+void check_no_tangent(const char *who, std::initializer_list<const at::Tensor *> tensors) {
+  for (const at::Tensor *t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(0).defined(), who, " has no forward-mode derivative (an input is a dual tensor)");
+}
+
 // the gradients of a node that is differentiable once: they say so when somebody differentiates them
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -101,6 +107,7 @@ void check_linear(const at::Tensor &x, const at::Tensor &w, const MaybeTensor &b
     for (int64_t i = 0; same && i + 1 < x.dim(); i++) same = res->size(i) == x.size(i);
     TORCH_CHECK_VALUE(same, "residual must have the shape of the output, rows of x by ", w.size(0), ", but got ", res->sizes());
   }
+  check_no_tangent("fused_linear", {&x, &w, bias ? &*bias : &x, res ? &*res : &x});
   for (const at::Tensor *t : {&x, &w, bias ? &*bias : &x, res ? &*res : &x}) {
     TORCH_CHECK_NOT_IMPLEMENTED(t->is_cuda(), "fused_linear runs on a HIP device only (a tensor is on ", t->device(), ")");
     TORCH_CHECK_VALUE(t->device() == x.device(), "x is on ", x.device(), ", another tensor on ", t->device());
@@ -233,6 +240,7 @@ void check_distill(const at::Tensor &s, const at::Tensor &v, const at::Tensor &i
     TORCH_CHECK_VALUE(rows, "weight must be floating, one number a row of the logits: got ", weight->scalar_type(), " of ", weight->sizes());
     TORCH_CHECK_VALUE(!weight->requires_grad(), "weight is a constant: no gradient reaches it");
   }
+  check_no_tangent("topk_distill_loss", {&s, weight ? &*weight : &s});
   for (const at::Tensor *t : {&s, &v, &i, weight ? &*weight : &s}) {
     TORCH_CHECK_NOT_IMPLEMENTED(t->is_cuda(), "topk_distill_loss runs on a HIP device only (a tensor is on ", t->device(), ")");
     TORCH_CHECK_VALUE(t->device() == s.device(), "logits are on ", s.device(), ", another tensor on ", t->device());

@@ -30,7 +30,7 @@ def topk_distill_loss(logits, teacher_values, teacher_indices, temperature=1.0, 
         0 have loss and gradient 0, whatever their logits hold.
 
     TypeError: a type that is not served; ValueError: shapes or numbers that do not fit, a weight that wants a gradient;
-    NotImplementedError: a tensor that is not on a HIP device.
+    NotImplementedError: a tensor that is not on a HIP device, dual logits or weights (there is no forward-mode derivative).
     """
     temperature = float(temperature)
     if not 1e-6 <= temperature <= 1e6:

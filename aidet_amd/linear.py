@@ -32,7 +32,7 @@ def fused_linear(x, weight, bias=None, residual=None, act='none'):
     All tensors are of one type (float32, bfloat16 or float16) and on one HIP device; under ``torch.autocast`` they are cast
     to its type first, as those of ``torch.nn.functional.linear`` are.  Differentiable once with respect to
     every tensor.  TypeError: a type that is not served, or several; ValueError: shapes that do not fit, an unknown act;
-    NotImplementedError: a tensor that is not on a HIP device.
+    NotImplementedError: a tensor that is not on a HIP device, or a dual tensor (there is no forward-mode derivative).
     """
     return torch_ext.ext().fused_linear(x, weight, bias, residual, _act_code(act))
 

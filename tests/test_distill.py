@@ -120,6 +120,24 @@ def test_wrapper_refusals(args, kwargs, error):
         topk_distill_loss(*args, **kwargs)
 
 
+@pytest.mark.parametrize('device', ['cpu', pytest.param(DEV, marks=pytest.mark.gpu)])
+def test_refuses_dual_tensors(device):
+    """logits or weights that are dual tensors; the teacher's values are a constant in forward mode too"""
+    import torch.autograd.forward_ad as fwad
+    from aidet_amd import topk_distill_loss
+    logits, values, weight = (torch.ones(*s, device=device) for s in ((3, 4), (3, 2), (3, )))
+    indices = torch.arange(2, device=device).expand(3, 2)
+    for grad in (True, False):
+        with fwad.dual_level(), torch.set_grad_enabled(grad):
+            def dual(t):
+                return fwad.make_dual(t, torch.ones_like(t))
+            for args in ((dual(logits), values, indices, 1., weight), (logits, values, indices, 1., dual(weight))):
+                with pytest.raises(NotImplementedError, match='forward-mode'):
+                    topk_distill_loss(*args)
+            if device != 'cpu':
+                assert torch.equal(topk_distill_loss(logits, dual(values), indices, 1., weight), topk_distill_loss(logits, values, indices, 1., weight))
+
+
 def test_c_abi_refusals_without_gpu():
     from aidet_amd import _lib
     L = _lib.lib()

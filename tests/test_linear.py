@@ -132,6 +132,36 @@ def test_wrapper_refusals(args, error):
         fused_linear(*args)
 
 
+def _dual_is_refused(device, match):
+    """every argument a dual tensor in turn, with and without grad mode"""
+    import torch.autograd.forward_ad as fwad
+    from aidet_amd import fused_linear
+    base = [torch.ones(*s, device=device) for s in ((3, 4), (5, 4), (5, ), (3, 5))]
+    for i in range(4):
+        for grad in (True, False):
+            with fwad.dual_level(), torch.set_grad_enabled(grad):
+                args = list(base)
+                args[i] = fwad.make_dual(base[i], torch.ones_like(base[i]))
+                with pytest.raises(NotImplementedError, match=match):
+                    fused_linear(*args)
+
+
+def test_refuses_dual_tensors():
+    _dual_is_refused('cpu', 'forward-mode')
+
+
+@pytest.mark.gpu
+def test_refuses_dual_tensors_on_the_device():
+    from aidet_amd import fused_linear
+    _dual_is_refused(DEV, 'forward-mode')
+    _dual_is_refused(DEV, 'fused_linear')
+    x, w, b, _ = make(3, 4, 5, torch.float32, True, False)
+    check(x, w, b, None, 'silu')                # (and afterwards it serves)
+    with torch.autocast('cuda', dtype=torch.bfloat16):
+        _dual_is_refused(DEV, 'forward-mode')
+        assert fused_linear(x, w).dtype == torch.bfloat16
+
+
 def test_c_abi_refusals_without_gpu():
     from aidet_amd import _lib
     L = _lib.lib()
