@@ -6,9 +6,9 @@
 // 2^-23 |x y| together, where one rounding of the fp32 product is 2^-24.  Six bf16 products, exact and added in fp32 by the
 // matrix unit, take 6 / 16 of the fp32 matrix instruction's time.  (bf16 has fp32's exponents and the matrix unit keeps
 // denormals: parts vanish only below 2^-133.)
-// Where a part overflows -- x infinite, or within 2^-9 of the largest number -- x - h is not finite and the sum is a NaN: a
-// workgroup that finds NaNs in its sums computes those again with the fp32 matrix instruction, whose infinities and NaNs are
-// IEEE's.
+// Where a part overflows -- x infinite, or within 2^-9 of the largest number -- x - h is not finite and the sum is a NaN; where h h
+// overflows and x y does not, the sum is infinite.  A workgroup that finds sums that are not finite computes those again with
+// the fp32 matrix instruction, whose infinities and NaNs are IEEE's.
 // What bounds it: 4096^3 615 us = 224 TFLOP/s (the fp32 matrix instruction's library product: 154), matrix pipe busy 66 % at
 // 1.96 GHz; the rest is splitting (two vector instructions a matrix instruction) and the two barriers of a step.
 #include "obb_linear_internal.h"
@@ -19,6 +19,8 @@ namespace lin {
 constexpr int BK = 32;      // k of a step: rows of 32 fp32 = a cache line; of 32 bf16 = 64 bytes in each of the three planes
 
 __device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
@@ -245,7 +247,7 @@ __global__ __launch_bounds__(256, B == 128 ? 2 : 3) void gemm_split_kernel(Gemm<
 #pragma unroll
       for (int j = 0; j < F; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) bad |= acc[i][j][e] != acc[i][j][e];
+        for (int e = 0; e < 4; e++) bad |= !finite(acc[i][j][e]);
     if (__syncthreads_or(bad)) {
       f32x4 ieee[F][F] = {};
 #pragma unroll 1
@@ -266,13 +268,13 @@ __global__ __launch_bounds__(256, B == 128 ? 2 : 3) void gemm_split_kernel(Gemm<
 #pragma unroll
           for (int j = 0; j < F; j++) ieee[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j], a[i], ieee[i][j], 0, 0, 0);
       }
-      // (only the NaN ones are exchanged: what a row gives does not hang on its neighbours)
+      // (only the ones that are not finite are exchanged: what a row gives does not hang on its neighbours)
 #pragma unroll
       for (int i = 0; i < F; i++)
 #pragma unroll
         for (int j = 0; j < F; j++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) acc[i][j][e] = acc[i][j][e] != acc[i][j][e] ? ieee[i][j][e] : acc[i][j][e];
+          for (int e = 0; e < 4; e++) acc[i][j][e] = finite(acc[i][j][e]) ? acc[i][j][e] : ieee[i][j][e];
     }
   }
   if (early) {

@@ -451,6 +451,34 @@ def test_activations_at_infinity(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('m', [33, 140])
+def test_fp32_products_next_to_the_largest_number(m):
+    """factors that 8 bits round up to the next power of two: the rounded ones' product overflows where the product does not.
+    One term a sum, the other factor a power of two: exact; then terms that add up to less than the largest number, in any order."""
+    from aidet_amd import fused_linear
+    g = torch.Generator(device=DEV).manual_seed(37)
+    x, w = torch.zeros(m, 200, device=DEV), torch.zeros(140, 200, device=DEV)
+    x[:, 7] = ((2 - 2.0 ** -9 * torch.rand(m, generator=g, device=DEV).double()) * 2.0 ** 63).float()
+    x[0, 7], x[1::2, 7] = 1.998 * 2.0 ** 63, -x[1::2, 7]
+    w[:, 7] = 2.0 ** 64 * (1 - 2 * (torch.arange(140, device=DEV) % 3 == 0).float())
+    want = (x[:, 7:8].double() * w[:, 7].double()).float()
+    assert bool(want.isfinite().all()) and torch.equal(fused_linear(x, w), want)
+    leaf = w.clone().requires_grad_(True)                   # (the gradients' products too: dy @ w, dy^T @ x)
+    dw, = torch.autograd.grad(fused_linear(x, leaf), leaf, torch.ones(m, 140, device=DEV) * 2.0 ** -20)
+    assert bool(dw.isfinite().all())
+    xl = torch.ones(m, 200, device=DEV, requires_grad=True)
+    dy = torch.zeros(m, 140, device=DEV)
+    dy[:, 3] = x[:, 7]
+    dx, = torch.autograd.grad(fused_linear(xl, w), xl, dy)
+    assert torch.equal(dx[:, 7], (x[:, 7].double() * w[3, 7].double()).float())
+    x[:, 8:12], w[:, 8:12] = x[:, 7:8] / 16, w[:, 7:8] * -1
+    check(x, w, None, None, 'none')
+    x[0, 20], w[1, 20] = float('inf'), 0.                  # (an infinite operand in the same tile, beside them)
+    y = fused_linear(x, w)
+    assert bool(y[0].isnan().all()) and bool(y[1:].isfinite().all())
+
+
+@pytest.mark.gpu
 def test_pitches_past_32_bits():
     """rows 2^31 and more elements apart"""
     from aidet_amd import fused_linear
