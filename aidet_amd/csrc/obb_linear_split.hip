@@ -1,15 +1,16 @@
 // obb_linear_split.hip -- the tiled product of fp32 operands on the bf16 matrix instructions.
 //
-// An fp32 number is the exact sum of three bf16 numbers (24 = 8 + 8 + 8 significant bits):
+// Times 2^16, which is exact, an fp32 number is the exact sum of three bf16 numbers (24 = 8 + 8 + 8 significant bits):
 //   h = x rounded to 8 bits,  m = x - h rounded to 8 bits,  l = the rest, exact       (|m| <= 2^-8 |h|, |l| <= 2^-8 |m|)
 // and x y = hh + (hm + mh) + (hl + lh + mm) + (ml + lm + ll).  The last three are left out: of either sign and at most
 // 2^-23 |x y| together, where one rounding of the fp32 product is 2^-24.  Six bf16 products, exact and added in fp32 by the
-// matrix unit, take 6 / 16 of the fp32 matrix instruction's time.  (bf16 has fp32's exponents and the matrix unit keeps
-// denormals: parts vanish only below 2^-133.)
-// Where a part overflows -- x infinite, or within 2^-9 of the largest number -- x - h is not finite and the sum is a NaN; where h h
-// overflows and x y does not, the sum is infinite.  A workgroup that finds sums that are not finite computes those again with
-// the fp32 matrix instruction, whose infinities and NaNs are IEEE's.
-// What bounds it: 4096^3 615 us = 224 TFLOP/s (the fp32 matrix instruction's library product: 154), matrix pipe busy 66 % at
+// matrix unit, take 6 / 16 of the fp32 matrix instruction's time.  The power of two is for small numbers: bf16 has fp32's exponents
+// but ends at 2^-133 (the matrix unit keeps denormals), fp32 at 2^-149, and an operand of 2^-120 without it kept 13 of its
+// bits.  The sums are 2^32 times too large until they leave.
+// Where a part or a sum overflows -- |x| from 2^112 on, infinite ones too, products and sums from 2^96 on -- the sum is infinite or a
+// NaN.  A workgroup that finds such sums computes those again with the fp32 matrix instruction, whose range, infinities and
+// NaNs are IEEE's.
+// What bounds it: 4096^3 615 us = 224 TFLOP/s (597 without the two multiplications a pair; the fp32 matrix instruction's library product: 154), matrix pipe busy 66 % at
 // 1.96 GHz; the rest is splitting (two vector instructions a matrix instruction) and the two barriers of a step.
 #include "obb_linear_internal.h"
 
@@ -27,7 +28,8 @@ typedef float f32x2u __attribute__((ext_vector_type(2), aligned(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
-// the three parts of eight numbers, packed
+// the three parts of eight numbers times 2^16, packed
+constexpr float SCALE = 65536.f, UNSCALE = 1.f / SCALE / SCALE;
 struct Parts { u32x4 h, m, l; };
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   union { bf16x2 v; uint32_t u; } r;
@@ -38,8 +40,9 @@ __device__ __forceinline__ Parts split8(const float (&x)[8]) {
   Parts p;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    p.h[i] = pack(x[2 * i], x[2 * i + 1]);
-    const float ra = x[2 * i] - __uint_as_float(p.h[i] << 16), rb = x[2 * i + 1] - __uint_as_float(p.h[i] & 0xffff0000u);
+    const float a = x[2 * i] * SCALE, b = x[2 * i + 1] * SCALE;
+    p.h[i] = pack(a, b);
+    const float ra = a - __uint_as_float(p.h[i] << 16), rb = b - __uint_as_float(p.h[i] & 0xffff0000u);
     p.m[i] = pack(ra, rb);
     p.l[i] = pack(ra - __uint_as_float(p.m[i] << 16), rb - __uint_as_float(p.m[i] & 0xffff0000u));
   }
@@ -247,7 +250,10 @@ __global__ __launch_bounds__(256, B == 128 ? 2 : 3) void gemm_split_kernel(Gemm<
 #pragma unroll
       for (int j = 0; j < F; j++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) bad |= !finite(acc[i][j][e]);
+        for (int e = 0; e < 4; e++) {
+          bad |= !finite(acc[i][j][e]);
+          acc[i][j][e] *= UNSCALE;
+        }
     if (__syncthreads_or(bad)) {
       f32x4 ieee[F][F] = {};
 #pragma unroll 1

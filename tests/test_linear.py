@@ -479,6 +479,26 @@ def test_fp32_products_next_to_the_largest_number(m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('m, n', [(20, 140), (33, 140), (140, 200), (300, 70)])
+@pytest.mark.parametrize('small, large', [(2.0 ** -112, 2.0 ** 60), (2.0 ** -120, 2.0 ** 60), (2.0 ** -127, 2.0 ** 100), (2.0 ** -141, 2.0 ** 110),
+                                          (2.0 ** -60, 2.0 ** -40), (2.0 ** -126, 1.)])
+def test_fp32_products_of_small_numbers(small, large, m, n):
+    """operands down to denormal numbers times large ones, sums among them: the accuracy of fp32 products whichever kernel the
+    number of rows selects, and whichever operand is the small one; the gradients' products as well.  Outputs that are denormal themselves
+    (the last size) are off by half of their step more: 2^-150, within the allowance of the smallest normal number."""
+    g = torch.Generator(device=DEV).manual_seed(41)
+    k = 500
+    x = (torch.randn(m, k, generator=g, device=DEV).double() * small).float()
+    w = torch.randn(n, k, generator=g, device=DEV) * large
+    check(x, w, None, None, 'none')
+    check(w[:, :k], x, None, None, 'none')
+    check(x[:, 3:8], w[:, 3:8], None, None, 'none')
+    one = torch.ones(m, k, device=DEV)
+    check_gradients(one, w, None, None, 'none', (torch.randn(m, n, generator=g, device=DEV).double() * small).float())
+    check_gradients(x, torch.zeros_like(w), None, None, 'none', torch.randn(m, n, generator=g, device=DEV) * large)
+
+
+@pytest.mark.gpu
 def test_pitches_past_32_bits():
     """rows 2^31 and more elements apart"""
     from aidet_amd import fused_linear
