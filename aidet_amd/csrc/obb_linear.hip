@@ -130,7 +130,7 @@ int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
 // every run).  dz is rounded to the type once, as the two products take operands of the type; db sums what was not rounded.
 // Block (x, y): 64 columns, rows y, y + chunks, ... of a few dozen; 16-byte accesses, four rows under way a thread, or one where
 // four would leave the device short of workgroups (both kernels, us, four and one: 777 x 515 fp32 gelu 10.6, 7.6; 1024 x 1024
-// bf16 relu 7.7, 7.0); partial sums [chunk][n] in the workspace.  Larger ones are memory's: 8192 x 1024 fp32 silu 26.5 us = 3.8 TB/s.
+// bf16 relu 7.7, 7.0); partial sums [chunk][n] in the workspace.  Larger ones are memory's: 8192 x 1024 fp32 silu 24.8 us = 4.1 TB/s, gelu 26.7.
 constexpr int CS_COLS = 64;
 static int colsum_depth(int64_t m, int64_t n, int dtype) {      // rows under way a thread
   const int64_t rows = dtype == OBB_F32 ? 64 : 128;

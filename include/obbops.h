@@ -651,7 +651,7 @@ OBB_API int obb_roi_backward_gather_nhwc_f32(const float *grad_out_dev, int B, i
 #define OBB_F16 2
 #define OBB_ACT_NONE 0
 #define OBB_ACT_RELU 1
-#define OBB_ACT_GELU 2   /* z Phi(z), by erf */
+#define OBB_ACT_GELU 2   /* z Phi(z), Phi the normal distribution's (no tanh form) */
 #define OBB_ACT_SILU 3   /* z / (1 + exp(-z)) */
 #define OBB_LINEAR_FORWARD 0
 #define OBB_LINEAR_ACT_BACKWARD 1

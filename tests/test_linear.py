@@ -499,6 +499,63 @@ def test_fp32_products_of_small_numbers(small, large, m, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('split', [False, True])
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
+def test_activations_everywhere(act, dtype, split, cut):
+    """z from -13 to 8 (silu from -87), in every number of the type or densely: the activation to its own accuracy, relative to the
+    value, the tail too; z is exact here (a factor of 1, one term).  fp32: q is a polynomial of 1 u, five roundings of its sum that count,
+    reciprocal, exp2 and two products of at most 2 u each: 14 u; z - z q next to -1 is 1 - 0.34 / 0.16 of that.  The exponential of silu
+    alike, its root squared.  16 u.  16 bits: (16 + 3 z^2) u -- silu (16 + 3 |z|) u -- and half a step of the type.  And in fp32 the error of normal
+    inputs is no larger than that of the elementary form, 0.5 z (1 + erf(z / sqrt 2)) and z / (1 + exp(-z)), but a tenth."""
+    from aidet_amd import fused_linear
+    low = -13 if act == 'gelu' else -87
+    if dtype == torch.float32:
+        z = torch.cat([torch.linspace(low, 8, 40001, device=DEV), torch.linspace(-0.05, 0.05, 4000, device=DEV)])
+    else:
+        z = torch.arange(-32768, 32768, device=DEV).to(torch.int16).view(dtype)
+        z = z[(z.float() >= low) & (z.float() <= 8)]
+    k = 256 if split else 1
+    cut(64, 2) if split else None
+    x, w = torch.zeros(z.numel(), k, device=DEV, dtype=dtype), torch.zeros(8, k, device=DEV, dtype=dtype)
+    x[:, 0], w[:, 0] = z, 1.
+    y = fused_linear(x, w, None, None, act)
+    assert bool((y == y[:, :1]).all())
+    got, d = y[:, 0].double(), z.double()
+    want = act64(d, act)
+    own = 16 * U if dtype == torch.float32 else (16 + 3 * (d * d if act == 'gelu' else d.abs())) * U + half_step(dtype)
+    step = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126      # (half a step of fp16; the exponentials end at the smallest normal number)
+    off = (got - want).abs() - own * want.abs() - step
+    assert bool((off <= 0).all()), (float(z[off.argmax()]), float(off.max()))
+    if dtype == torch.float32:
+        z = torch.randn(1 << 18, 1, generator=torch.Generator(device=DEV).manual_seed(43), device=DEV)
+        plain = 0.5 * z * (1 + torch.erf(z * 0.5 ** 0.5)) if act == 'gelu' else z / (1 + torch.exp(-z))
+        want = act64(z.double(), act)
+        x = torch.zeros(1 << 18, k, device=DEV)
+        x[:, :1] = z
+        got = fused_linear(x, w, None, None, act)[:, :1]
+        off, off_plain = ((((t.double() - want) / want) ** 2).mean().sqrt() for t in (got, plain))
+        assert float(off) <= 1.1 * float(off_plain), (float(off), float(off_plain))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('act', ['gelu', 'silu'])
+def test_slopes_everywhere(act):
+    """the slope over the same range, fp32: 8 u absolute, and 8 u (1 + z^2) of z's size times the density in the tail"""
+    z = torch.linspace(-13, 8, 40001, device=DEV)[:, None]
+    r = z.clone().requires_grad_(True)
+    from aidet_amd import fused_linear
+    y = fused_linear(torch.zeros(z.numel(), 1, device=DEV), torch.zeros(1, 1, device=DEV), None, r, act)
+    got, = torch.autograd.grad(y, r, torch.ones_like(y))
+    d = z.double()
+    off = (got.double() - slope64(d, act)).abs()
+    assert float(off.max()) <= 8 * U
+    tail = d < -5
+    size = d.abs() * torch.exp(-d * d / 2) if act == 'gelu' else d.abs() * torch.exp(d)
+    assert bool((off[tail] <= (8 * U * (1 + d * d) * size)[tail]).all())
+
+
+@pytest.mark.gpu
 def test_pitches_past_32_bits():
     """rows 2^31 and more elements apart"""
     from aidet_amd import fused_linear
