@@ -61,6 +61,12 @@ def _channels_last(x):
     return x.is_cuda and x.is_contiguous(memory_format=torch.channels_last)
 
 
+def _bare(*layers):
+    """Whether a fused layer may stand in for these: nothing hangs on their own calls (no hooks) and their forward is torch's."""
+    return all(not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks)
+               and type(m).forward in (nn.Linear.forward, nn.Conv2d.forward, nn.BatchNorm2d.forward) for m in layers)
+
+
 class Bottleneck(nn.Module):
     expansion = 4
 
@@ -104,7 +110,7 @@ class Bottleneck(nn.Module):
     def forward(self, x):
         if self.folded and (self.training or self.bn1.training or self.bn3.training):
             self.fold(False)        # (a norm in training mode goes by the batch, and moves the statistics that were folded)
-        if self.folded and not torch.is_grad_enabled() and _channels_last(x):
+        if self.folded and not torch.is_grad_enabled() and _channels_last(x) and _bare(self.conv1, self.bn1, self.conv3, self.bn3):
             idt = x if self.downsample is None else self.downsample(x)
             out = F.relu(self.bn2(self.conv2(pointwise(x, self.w1, self.b1, act='relu'))), inplace=True)
             return pointwise(out, self.w3, self.b3, idt, 'relu')
@@ -157,7 +163,10 @@ class FPN(nn.Module):
         for i in range(len(inputs) - 1, -1, -1):
             conv = self.lateral_convs[i]
             up = None if lat[-1] is None else F.interpolate(lat[i + 1], size=inputs[i].shape[2:], mode='nearest')
-            lat[i] = pointwise(inputs[i], conv.weight.flatten(1), conv.bias, up)
+            if _bare(conv):
+                lat[i] = pointwise(inputs[i], conv.weight.flatten(1), conv.bias, up)
+            else:
+                lat[i] = conv(inputs[i]) if up is None else conv(inputs[i]) + up
         return lat
 
     def forward(self, inputs):
@@ -221,13 +230,12 @@ class SharedFCHead(nn.Module):
 
     def forward(self, x):
         x = x.flatten(1)
-        if self.fused_linear:
-            for fc in self.shared_fcs:
-                x = fused_linear(x, fc.weight, fc.bias, act='relu')
-            return fused_linear(x, self.fc_cls.weight, self.fc_cls.bias), fused_linear(x, self.fc_reg.weight, self.fc_reg.bias)
         for fc in self.shared_fcs:
-            x = F.relu(fc(x))
-        return self.fc_cls(x), self.fc_reg(x)
+            x = fused_linear(x, fc.weight, fc.bias, act='relu') if self._fused(fc) else F.relu(fc(x))
+        return tuple(fused_linear(x, fc.weight, fc.bias) if self._fused(fc) else fc(x) for fc in (self.fc_cls, self.fc_reg))
+
+    def _fused(self, fc):
+        return self.fused_linear and _bare(fc)
 
     def distill_loss(self, x, teacher_values, teacher_indices, temperature=1.0, label_weights=None, avg_factor=None):
         """Loss of this head's class logits for the pooled RoIs `x` against a teacher's top logits of the same RoIs

@@ -114,6 +114,77 @@ def test_training_mode_and_loading_end_the_folding_of_the_whole_detector(calls):
     assert on() == {True}
 
 
+def test_layers_with_hooks_of_their_own_are_called(calls, monkeypatch):
+    """a hook of any kind on a layer, or a layer of another class in its place: that layer is called as a module, the others stay
+    fused; without hooks none is called"""
+    import aidet_amd.models.theta_obb_rcnn as mod
+    nn = torch.nn
+    rows = []
+
+    def plain(x, weight, bias=None, residual=None, act='none'):
+        rows.append(tuple(weight.shape))
+        y = nn.functional.linear(x, weight, bias)
+        return y.relu() if act == 'relu' else y
+    monkeypatch.setattr(mod, 'fused_linear', plain)
+    torch.manual_seed(5)
+
+    def hooked(layer, kind):
+        seen = []
+        register = getattr(layer, 'register_' + kind)
+        return seen, register(lambda m, *a: seen.append(m) and None)
+    # heads
+    head = mod.SharedFCHead(5, in_channels=2, fc_out_channels=8, fused_linear=True)
+    x = torch.randn(3, 2, 7, 7)
+    want = head(x)
+    assert len(rows) == 4
+    for kind in ('forward_hook', 'forward_pre_hook', 'full_backward_hook', 'full_backward_pre_hook'):
+        for layer in (head.shared_fcs[0], head.shared_fcs[1], head.fc_cls, head.fc_reg):
+            rows.clear()
+            seen, handle = hooked(layer, kind)
+            got = head(x)
+            sum(g.sum() for g in got).backward()
+            handle.remove()
+            assert seen == [layer] and len(rows) == 3
+            assert all(torch.allclose(g, w, atol=1e-6) for g, w in zip(got, want))
+
+    class Doubled(nn.Linear):
+        def forward(self, x):
+            return 2 * super(Doubled, self).forward(x)
+    rows.clear()
+    first = head.shared_fcs[0]
+    head.shared_fcs[0] = Doubled(98, 8)
+    head.shared_fcs[0].load_state_dict({k: v / 2 for k, v in first.state_dict().items()})
+    assert all(torch.allclose(g, w, atol=1e-6) for g, w in zip(head(x), want)) and len(rows) == 3
+    # bottlenecks
+    block = mod.Bottleneck(16, 4).eval()
+    block.fold()
+    x = torch.randn(1, 16, 5, 6)
+    with torch.no_grad():
+        want = block(x)
+        assert len(calls) == 2
+        for kind in ('forward_hook', 'forward_pre_hook'):
+            for layer in (block.conv1, block.bn1, block.conv3, block.bn3):
+                calls.clear()
+                seen, handle = hooked(layer, kind)
+                got = block(x)
+                handle.remove()
+                assert seen == [layer] and not calls and torch.allclose(got, want, atol=1e-5)
+        assert block.folded and torch.equal(block(x), want)
+    # pyramid
+    neck = mod.FPN((3, 4, 5), 6, 4)
+    neck.fused_linear = True
+    feats = [torch.randn(1, c, 16 >> i, 16 >> i) for i, c in enumerate((3, 4, 5))]
+    calls.clear()
+    want = neck(feats)
+    assert len(calls) == 3
+    for layer in neck.lateral_convs:
+        calls.clear()
+        seen, handle = hooked(layer, 'forward_hook')
+        got = neck(feats)
+        handle.remove()
+        assert seen == [layer] and len(calls) == 2 and all(torch.allclose(g, w, atol=1e-5) for g, w in zip(got, want))
+
+
 @pytest.mark.gpu
 def test_heads_on_fused_layers():
     from aidet_amd.models.theta_obb_rcnn import SharedFCHead
