@@ -424,7 +424,29 @@ template <typename T, bool FORWARD> static bool short_rows(const Args &a, hipStr
   return false;
 }
 
+// Rows r0 ... r0 + n - 1 of a call.  A launch has fewer than 2^32 threads (the runtime cuts a larger one short without an error) and a row
+// takes up to 256 of them: calls of more than ROWS rows go in several.
+constexpr int64_t ROWS = 1 << 23;
+template <typename T> static Args rows_of(const Args &a, int64_t r0, int64_t n) {
+  Args b = a;
+  b.rows = n;
+  b.logits = (const T *)a.logits + r0 * a.ld;
+  b.values = (const char *)a.values + r0 * a.k * (a.vtype == OBB_F32 ? 4 : 2);
+  b.indices = (const char *)a.indices + r0 * a.k * (a.wide_index ? 8 : 4);
+  if (a.weight) b.weight = a.weight + r0;
+  if (a.loss) b.loss = a.loss + r0;
+  if (a.stats) b.stats = a.stats + r0;
+  if (a.grad) b.grad = a.grad + r0 * a.grad_stride;
+  if (a.dlogits) b.dlogits = (T *)a.dlogits + r0 * a.ldd;
+  return b;
+}
+
 template <typename T> static int forward(const Args &a, float2 *ws, hipStream_t st) {
+  if (a.rows > ROWS) {
+    for (int64_t r0 = 0; r0 < a.rows; r0 += ROWS)
+      if (int rc = forward<T>(rows_of<T>(a, r0, a.rows - r0 < ROWS ? a.rows - r0 : ROWS), ws, st)) return rc;
+    return OBB_OK;
+  }
   if (!short_rows<T, true>(a, st)) {
     const int parts = parts_of(a.rows, a.classes);
     if (parts == 1) {
@@ -442,27 +464,24 @@ template <typename T> static int forward(const Args &a, float2 *ws, hipStream_t 
   return OBB_OK;
 }
 
-template <typename T> static int backward(Args a, hipStream_t st) {
+template <typename T> static int backward(const Args &a, hipStream_t st) {
+  if (a.rows > ROWS) {                                // (the last rows first, as within a launch)
+    for (int64_t end = a.rows; end > 0; end -= end < ROWS ? end : ROWS)
+      if (int rc = backward<T>(rows_of<T>(a, end < ROWS ? 0 : end - ROWS, end < ROWS ? end : ROWS), st)) return rc;
+    return OBB_OK;
+  }
   if (!short_rows<T, false>(a, st)) {
     const int parts = parts_of(a.rows, a.classes);
     const int64_t per = parts == 1 ? a.classes : ((a.classes + parts - 1) / parts + 7) / 8 * 8;
-    // (a grid's second dimension ends at 65535: more rows go in several launches, the last rows first)
+    // (a grid's second dimension ends at 65535: more rows go in several launches)
     for (int64_t end = a.rows; end > 0;) {
-      const int64_t n = end < 65535 ? end : 65535, r0 = end - n;
-      Args b = a;
-      b.rows = n;
-      b.logits = (const T *)a.logits + r0 * a.ld;
-      b.dlogits = (T *)a.dlogits + r0 * a.ldd;
-      b.values = (const char *)a.values + r0 * a.k * (a.vtype == OBB_F32 ? 4 : 2);
-      b.indices = (const char *)a.indices + r0 * a.k * (a.wide_index ? 8 : 4);
-      b.weight = a.weight ? a.weight + r0 : nullptr;
-      b.stats = a.stats + r0;
-      b.grad = a.grad + r0 * a.grad_stride;
+      const int64_t n = end < 65535 ? end : 65535;
+      const Args b = rows_of<T>(a, end - n, n);
       if (parts == 1 && a.classes <= WAVE_ROW && a.k <= 256) distill_backward_kernel<T, 64, 256><<<dim3(1, (unsigned)n), 64, 0, st>>>(b, per);
       else if (a.k <= 256) distill_backward_kernel<T, 256, 256><<<dim3(parts, (unsigned)n), 256, 0, st>>>(b, per);
       else distill_backward_kernel<T, 256, KMAX><<<dim3(parts, (unsigned)n), 256, 0, st>>>(b, per);
       OBB_LAUNCH_CHECK();
-      end = r0;
+      end -= n;
     }
   }
   OBB_LAUNCH_CHECK();

@@ -43,7 +43,7 @@ int join_splits(const Gemm<T> &g, const float *partial, int splits, hipStream_t 
   const int64_t per_row = (g.n + 7) / 8, all = g.m * per_row;
   const int threads = all < 256 * 256 ? 64 : 256;
   const int64_t blocks = (all + threads - 1) / threads;
-  if (blocks > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many blocks");
+  if (int rc = check_launch(blocks, threads)) return rc;
   if (splits > 8) join_splits_kernel<T, 16><<<(unsigned)blocks, threads, 0, stream>>>(g, partial, splits, (uint32_t)per_row);
   else join_splits_kernel<T, 8><<<(unsigned)blocks, threads, 0, stream>>>(g, partial, splits, (uint32_t)per_row);
   OBB_LAUNCH_CHECK();
@@ -253,6 +253,7 @@ static int act_backward(const void *dy, const void *y, const float *z, int64_t m
                         void *ws, hipStream_t stream) {
   const int chunks = colsum_chunks(m, n, sizeof(T) == 4 ? OBB_F32 : OBB_BF16);
   float *partial = db ? (float *)ws : nullptr;
+  if (int rc = check_launch((n + CS_COLS - 1) / CS_COLS, 256)) return rc;
   const dim3 grid((unsigned)((n + CS_COLS - 1) / CS_COLS), chunks);
   if (colsum_depth(m, n, sizeof(T) == 4 ? OBB_F32 : OBB_BF16) == 1)
     act_backward_kernel<T, 1><<<grid, 256, 0, stream>>>((const T *)dy, (const T *)y, z, m, n, act, (T *)dz, partial);

@@ -251,6 +251,13 @@ __device__ __forceinline__ void tile_out(const Gemm<T> &g, const f32x4 (&acc)[FM
   }
 }
 
+// A dimension of a launch has fewer than 2^32 threads; the runtime cuts a larger one short without an error.
+inline int check_launch(int64_t blocks, int threads) {
+  if (blocks > 0xffffffffll / threads)
+    return set_err(OBB_EINVAL, "obb_linear: the output is too large for one launch (%lld workgroups of %d threads, fewer than 2^32 threads fit)", (long long)blocks, threads);
+  return OBB_OK;
+}
+
 // the splits' sums, joined in their order, and the epilogue
 template <typename T> int join_splits(const Gemm<T> &g, const float *partial, int splits, hipStream_t stream);
 

@@ -307,7 +307,7 @@ __global__ __launch_bounds__(256) void gemm_ragged_kernel(Gemm<T> g, uint32_t ti
 template <typename T, int B, bool TA, bool TB>
 static int launch_ragged(const Gemm<T> &g, int splits, float *partial, hipStream_t stream) {
   const int64_t tm = (g.m + B - 1) / B, tn = (g.n + B - 1) / B, slabs = (g.k + BK - 1) / BK, per = (slabs + splits - 1) / splits;
-  if (tm * tn * splits > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many tiles (%lld x %lld)", (long long)tm, (long long)tn);
+  if (int rc = check_launch(tm * tn * splits, 256)) return rc;
   const uint32_t grid = (uint32_t)(tm * tn * splits), um = (uint32_t)tm, un = (uint32_t)tn, us = (uint32_t)splits;
   const int act = splits > 1 ? OBB_ACT_NONE : g.act;
   if constexpr (!TA && !TB) {
@@ -336,7 +336,7 @@ static int launch_act(const Gemm<T> &g, uint32_t tm, uint32_t tn, uint32_t split
 template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB>
 static int launch(const Gemm<T> &g, int splits, float *partial, hipStream_t stream) {
   const int64_t tm = (g.m + BM - 1) / BM, tn = (g.n + BN - 1) / BN, slabs = (g.k + BK - 1) / BK, per = (slabs + splits - 1) / splits;
-  if (tm * tn * splits > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many tiles (%lld x %lld)", (long long)tm, (long long)tn);
+  if (int rc = check_launch(tm * tn * splits, WM * WN * 64)) return rc;
   const int act = splits > 1 ? OBB_ACT_NONE : g.act;
   if constexpr (!TA && !TB) {                        // (the gradients' products have no activation)
     if (act == OBB_ACT_RELU) return launch_act<T, BM, BN, WM, WN, TA, TB, OBB_ACT_RELU>(g, (uint32_t)tm, (uint32_t)tn, splits, per, partial, stream);

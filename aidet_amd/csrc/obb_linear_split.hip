@@ -296,7 +296,7 @@ __global__ __launch_bounds__(256, B == 128 ? 2 : 3) void gemm_split_kernel(Gemm<
 template <int B, bool TA, bool TB>
 static int launch_split(const Gemm<float> &g, int splits, float *partial, hipStream_t stream) {
   const int64_t tm = (g.m + B - 1) / B, tn = (g.n + B - 1) / B, steps = (g.k + BK - 1) / BK, per = (steps + splits - 1) / splits;
-  if (tm * tn * splits > 0x7fffffff) return set_err(OBB_EINVAL, "obb_linear: too many tiles (%lld x %lld)", (long long)tm, (long long)tn);
+  if (int rc = check_launch(tm * tn * splits, 256)) return rc;
   const uint32_t grid = (uint32_t)(tm * tn * splits), um = (uint32_t)tm, un = (uint32_t)tn;
   const int act = splits > 1 ? OBB_ACT_NONE : g.act;
   if constexpr (!TA && !TB) {

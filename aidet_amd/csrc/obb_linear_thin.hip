@@ -99,6 +99,7 @@ template <typename T, int FM>
 static int launch(const Gemm<T> &g, hipStream_t stream) {
   const int64_t blocks = (g.n + 15) / 16, steps = (g.k * (int64_t)sizeof(T) + 64 * DEPTH - 1) / (64 * DEPTH);
   const unsigned threads = 64 * (unsigned)(steps < 1 ? 1 : steps < WAVES ? steps : WAVES);
+  if (int rc = check_launch(blocks, (int)threads)) return rc;
   if (g.act == OBB_ACT_RELU) gemm_thin_kernel<T, FM, OBB_ACT_RELU><<<(unsigned)blocks, threads, 0, stream>>>(g);
   else if (g.act == OBB_ACT_GELU) gemm_thin_kernel<T, FM, OBB_ACT_GELU><<<(unsigned)blocks, threads, 0, stream>>>(g);
   else if (g.act == OBB_ACT_SILU) gemm_thin_kernel<T, FM, OBB_ACT_SILU><<<(unsigned)blocks, threads, 0, stream>>>(g);

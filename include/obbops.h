@@ -635,7 +635,8 @@ OBB_API int obb_roi_backward_gather_nhwc_f32(const float *grad_out_dev, int B, i
  *   z = x w^T + bias + res,  y = act(z);   dz = dy act'(z),  dx = dz w,  dw = dz^T x,  dbias = sum_m dz,  dres = dz
  * x (m, k) with row pitch ldx, w (n, k) with row pitch ldw, bias (n) or NULL, res (m, n) with row pitch ldr (0 = one row
  * for all) or NULL, y (m, n); all of one dtype (pitches in elements), products and sums in fp32, one rounding to the
- * dtype at the end.  Any sizes (zero too), pitches and element-aligned pointers; outputs must not overlap inputs.
+ * dtype at the end.  Any sizes (zero too; an output that would take a launch of 2^32 threads, from about 2^36 elements on, is
+ * OBB_EINVAL), pitches and element-aligned pointers; outputs must not overlap inputs.
  * Training: gelu and silu need the pre-activation, written to z (m, n) fp32 (NULL otherwise); relu needs y only.
  *   obb_linear_act_backward    dy (m, n) -> dz (m, n) of the dtype (NULL: not wanted; may be dy itself), dbias (n) (NULL: not wanted)
  *   obb_linear_backward_input  dz, w -> dx (m, k)          obb_linear_backward_weight  dz, x -> dw (n, k)

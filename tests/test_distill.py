@@ -318,6 +318,28 @@ def test_rows_past_32_bits():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('rows, classes, k', [((1 << 28) + 17, 2, 1), ((1 << 24) + 17, 65, 257)])
+def test_more_rows_than_a_launch_holds(rows, classes, k):
+    """a launch has fewer than 2^32 threads, 16 or 256 of them a row here: every row is served, with the bits of a small call"""
+    from aidet_amd import topk_distill_loss
+    g = torch.Generator(device=DEV).manual_seed(47)
+    logits = torch.empty(rows, classes, device=DEV, dtype=torch.float16)
+    few = torch.randn(1 << 16, classes, generator=g, device=DEV).half()
+    for r in range(0, rows, 1 << 16):                       # (rows repeat: 2^16 different ones, and a shift)
+        logits[r:r + (1 << 16)] = few[:rows - r]
+    values = torch.randn(1, k, generator=g, device=DEV).half().expand(rows, k)
+    indices = (torch.arange(k, device=DEV, dtype=torch.int32) % classes).expand(rows, k).contiguous()
+    logits.requires_grad_(True)
+    loss = topk_distill_loss(logits, values, indices, reduction='none')
+    grad, = torch.autograd.grad(loss, logits, torch.ones_like(loss))
+    want = topk_distill_loss(few, values[:1 << 16], indices[:1 << 16], reduction='none')
+    want_grad, = torch.autograd.grad(topk_distill_loss(few.requires_grad_(True), values[:1 << 16], indices[:1 << 16], reduction='sum'), few)
+    for r in range(0, rows, 1 << 16):
+        n = min(1 << 16, rows - r)
+        assert torch.equal(loss[r:r + n], want[:n]) and torch.equal(grad[r:r + n], want_grad[:n]), r
+
+
+@pytest.mark.gpu
 def test_against_differences():
     """fp32 against central differences of the plain form in 64 bits (h = 1e-5: good to ~1e-9)"""
     for rows, classes, k in ((6, 16, 4), (4, 1500, 40)):

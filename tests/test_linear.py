@@ -186,6 +186,21 @@ def test_c_abi_refusals_without_gpu():
     assert L.obb_linear_workspace_bytes(-1, 5, 4, 0, 0) == 0
 
 
+def test_c_abi_refuses_launches_past_the_limit():
+    """a dimension of a launch has fewer than 2^32 threads: a call that would need more says so"""
+    from aidet_amd import _lib
+    L = _lib.lib()
+    one, null, big = ctypes.c_void_p(256), None, 1 << 46     # (never dereferenced: refused before any launch)
+    wide = (1 << 31) - 1
+    for dtype in range(3):
+        for rc in (L.obb_linear_forward(one, 8, one, 8, null, null, 0, 1 << 33, 64, 8, dtype, 0, one, null, one, big, null),
+                   L.obb_linear_forward(one, 9, one, 9, null, null, 0, 40, wide, 9, dtype, 0, one, null, one, big, null),
+                   L.obb_linear_backward_input(one, one, 64, 1 << 33, 8, 64, dtype, one, one, big, null),
+                   L.obb_linear_backward_weight(one, one, 40, 8, wide, 40, dtype, one, one, big, null),
+                   L.obb_linear_act_backward(one, one, null, 3, wide, dtype, 1, one, one, one, big, null)):
+            assert rc == _lib.OBB_EINVAL and b'threads' in L.obb_last_error(), (dtype, rc, L.obb_last_error())
+
+
 @pytest.mark.parametrize('op', range(4))
 @pytest.mark.parametrize('dtype', range(3))
 def test_workspaces_of_empty_sizes(op, dtype):
