@@ -23,7 +23,8 @@ def topk_distill_loss(logits, teacher_values, teacher_indices, temperature=1.0, 
         temperature (float): T, from 1e-6 to 1e6
         weight (Tensor, optional): (...) weight per row, a constant
         reduction (str): 'none' | 'mean' | 'sum'
-        avg_factor (float, optional): with 'mean', the sum is divided by it instead of by the number of rows
+        avg_factor (float, optional): with 'mean', the sum is divided by it instead of by the number of rows ('none' is not
+            touched by it, 'sum' refuses it)
 
     Returns:
         fp32: the rows' losses (...) or a scalar (0 where there are no rows).  A row without an entry and a row of weight
@@ -39,11 +40,12 @@ def topk_distill_loss(logits, teacher_values, teacher_indices, temperature=1.0, 
         raise ValueError("reduction must be 'none', 'mean' or 'sum', but got {!r}".format(reduction))
     scale = -1. if reduction == 'none' else 1.
     if avg_factor is not None:
-        if reduction != 'mean':
+        if reduction == 'sum':
             raise ValueError("avg_factor goes with reduction='mean'")
         if not float(avg_factor) > 0:
             raise ValueError('avg_factor must be positive, but got {}'.format(avg_factor))
-        scale = 1. / float(avg_factor)
+        if reduction == 'mean':
+            scale = 1. / float(avg_factor)
     elif reduction == 'mean' and hasattr(logits, 'shape'):
         scale = 1. / max(logits.shape[:-1].numel(), 1)
     return torch_ext.ext().topk_distill(logits, teacher_values, teacher_indices, temperature, weight, scale)

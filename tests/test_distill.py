@@ -403,6 +403,27 @@ def test_module_follows_the_losses_conventions():
     assert m(logits, values, indices, reduction_override='none').shape == (12, )
 
 
+@pytest.mark.parametrize('device', ['cpu', pytest.param(DEV, marks=pytest.mark.gpu)])
+def test_avg_factor_of_unreduced_losses(device, monkeypatch):
+    """heads pass avg_factor whatever the reduction: 'none' leaves the rows' losses as they are, as the reference's losses do"""
+    from aidet_amd import TopkDistillLoss, topk_distill_loss, torch_ext
+    args = [torch.randn(5, 7, device=device), torch.randn(5, 2, device=device), torch.arange(2, device=device).expand(5, 2).contiguous()]
+    if device == 'cpu':
+        class Ext:
+            @staticmethod
+            def topk_distill(logits, values, indices, temperature, weight, scale):
+                return scale
+        monkeypatch.setattr(torch_ext, 'ext', Ext)
+        assert topk_distill_loss(*args, reduction='none', avg_factor=3.) == -1
+        assert topk_distill_loss(*args, reduction='mean', avg_factor=4.) == 0.25
+        return
+    want = topk_distill_loss(*args, reduction='none')
+    assert want.shape == (5, ) and torch.equal(topk_distill_loss(*args, reduction='none', avg_factor=3.), want)
+    assert torch.equal(TopkDistillLoss(loss_weight=0.5)(*args, avg_factor=3., reduction_override='none'), 0.5 * want)
+    with pytest.raises(ValueError):
+        topk_distill_loss(*args, reduction='sum', avg_factor=3.)
+
+
 @pytest.mark.gpu
 def test_a_head_learns_from_a_teachers_top_logits():
     """FC trunk, class logits, loss and gradients together: against the same chain in 64 bits.  Whole steps of fp32: the
