@@ -11,6 +11,8 @@
 #include <torch/csrc/autograd/graph_task.h>
 
 #include <tuple>
+#include <unordered_set>
+#include <vector>
 
 #include "obbops.h"
 
@@ -76,21 +78,32 @@ variable_list once(variable_list grads) {
 
 // A leaf's gradient is added up on the stream where its accumulator was made, and the accumulator lives as long as any graph
 // of the leaf.  One of the default stream, which takes no part in a capture, would end a process that captures this pass: say so.
+// All accumulators that this pass will reach from here are looked at, behind casts, views and other layers too.
 void check_capture(void *stream) {
   hipStreamCaptureStatus status;
   if (hipStreamIsCapturing((hipStream_t)stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
   const auto node = torch::autograd::get_current_node();
   const auto *exec = torch::autograd::get_current_graph_task_exec_info();
   if (!node) return;
-  for (const auto &edge : node->next_edges()) {
-    auto *leaf = dynamic_cast<torch::autograd::AccumulateGrad *>(edge.function.get());
-    if (!leaf) continue;
-    if (exec && !exec->empty()) {
-      const auto it = exec->find(leaf);
-      if (it == exec->end() || !it->second.should_execute()) continue;
+  std::vector<torch::autograd::Node *> todo = {node.get()};
+  std::unordered_set<torch::autograd::Node *> seen;
+  while (!todo.empty()) {
+    auto *at = todo.back();
+    todo.pop_back();
+    for (const auto &edge : at->next_edges()) {
+      auto *next = edge.function.get();
+      if (!next || !seen.insert(next).second) continue;
+      if (exec && !exec->empty()) {
+        const auto it = exec->find(next);
+        if (it == exec->end() || !it->second.should_execute()) continue;
+      }
+      if (dynamic_cast<torch::autograd::AccumulateGrad *>(next)) {
+        const auto s = next->stream();
+        TORCH_CHECK(!s || s->id() != 0, "a backward pass is captured while a graph of the same leaves from the default stream is alive: free that graph's outputs before the capture");
+      } else {
+        todo.push_back(next);
+      }
     }
-    const auto s = leaf->stream();
-    TORCH_CHECK(!s || s->id() != 0, "a backward pass is captured while a graph of the same leaves from the default stream is alive: free that graph's outputs before the capture");
   }
 }
 

@@ -850,3 +850,44 @@ def test_capture_beside_an_eager_graph_of_the_default_stream():
             assert torch.equal(leaf.grad, want)
         del kept
         leaf.grad = None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('way', ['autocast', 'view'])
+def test_capture_beside_an_eager_graph_whose_leaves_are_behind_other_nodes(way):
+    """the same where the leaf reaches the layer through a cast of autocast, or a product and a view"""
+    from aidet_amd import fused_linear
+    w = torch.randn(24, 40, device=DEV, requires_grad=True)
+    x = torch.randn(9, 40, device=DEV)
+
+    def loss():
+        if way == 'view':
+            return fused_linear(x, (w * 2).view(24, 40), act='silu').square().sum()
+        with torch.autocast('cuda', dtype=torch.bfloat16, cache_enabled=False):
+            return fused_linear(x, w, act='silu').float().square().sum()
+    kept = loss()
+    kept.backward()
+    want, w.grad = w.grad, None
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match='graph of the same leaves'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            loss().backward()
+    torch.cuda.synchronize()
+    del kept
+    w.grad = None
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        loss().backward()
+    torch.cuda.current_stream().wait_stream(s)
+    w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss().backward()
+    for _ in range(3):
+        w.grad.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(w.grad, want)
+    w.grad = None
