@@ -227,6 +227,44 @@ def test_pyramid_on_fused_layers():
 
 
 @pytest.mark.gpu
+def test_the_fused_paths_run(monkeypatch):
+    """channels-last tile: two fused layers a bottleneck and one a level, all by the kernel, where the detector is folded and none
+    where it is not; every head layer where the heads are fused; what they give is the unfused detector's within the layers' bound"""
+    import aidet_amd.models.theta_obb_rcnn as mod
+    made = []
+    kernel = mod.fused_linear
+
+    def counted(x, weight, *args, **kwargs):
+        made.append(tuple(weight.shape))
+        return kernel(x, weight, *args, **kwargs)
+    monkeypatch.setattr(mod, 'fused_linear', counted)
+    dev = torch.device(DEV)
+    models = [mod.build_detector(dev, fused_linear=f).to(memory_format=torch.channels_last) for f in (False, True)]
+    img, _ = mod.demo_inputs(dev, 256)
+    img = img.contiguous(memory_format=torch.channels_last)
+    with torch.no_grad():
+        want = models[0].extract_feat(img)
+        pooled = torch.randn(50, 256, 7, 7, device=dev)
+        heads = [h(pooled) for h in (models[0].bbox_head, models[0].rbbox_head)]
+        assert not made
+        got = models[1].fold_pointwise().extract_feat(img)
+        assert len(made) == 2 * 16 + 4
+        for g, w in zip(got, want):
+            _near(g, w, 16 * 3 + 2, 512)
+        made.clear()
+        for head, outs in zip((models[1].bbox_head, models[1].rbbox_head), heads):
+            for g, w in zip(head(pooled), outs):
+                _near(g, w, 3, 12544)
+        assert len(made) == 8
+        made.clear()
+        models[1].fold_pointwise(False).extract_feat(img)
+        assert not made
+        # (the convolutions of a model that is not channels-last give maps that are not, and are served by themselves)
+        mod.build_detector(dev).fold_pointwise().extract_feat(img.contiguous())
+        assert not made
+
+
+@pytest.mark.gpu
 def test_detector_tile_on_fused_layers():
     from aidet_amd.models import build_detector, demo_inputs
     dev = torch.device(DEV)
