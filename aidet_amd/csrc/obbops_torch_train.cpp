@@ -34,6 +34,10 @@ int64_t leading(const at::Tensor &t) {
   return n;
 }
 
+// A tensor whose sign waits to be turned -- the imaginary part of a conjugate -- is turned: the kernels read memory.
+at::Tensor turned(const at::Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+MaybeTensor turned(const MaybeTensor &t) { return t && t->is_neg() ? MaybeTensor(t->resolve_neg()) : t; }
+
 // (..., cols) as rows that the kernels read in place; copied only where the last dimension is not contiguous or rows overlap
 struct Rows {
   at::Tensor t;
@@ -185,7 +189,7 @@ struct FusedLinear : public torch::autograd::Function<FusedLinear> {
       void *stream = stream_of(x);
       check_capture(stream);
       const int code = code_of(x.scalar_type());
-      const at::Tensor dy = grads[0].contiguous();
+      const at::Tensor dy = turned(grads[0]).contiguous();
       at::Tensor dz = dy;
       const bool want_dz = act != OBB_ACT_NONE && (need & 11);
       if (want_dz) dz = at::empty_like(dy);
@@ -227,7 +231,9 @@ at::Tensor linear(const at::Tensor &x, const at::Tensor &w, const MaybeTensor &b
 // under autocast the tensors are cast as those of torch's own linear layer are
 at::Tensor cast(const at::Tensor &t, at::ScalarType type) { return code_of(t.scalar_type()) >= 0 ? t.to(type) : t; }
 
-at::Tensor fused_linear(const at::Tensor &x, const at::Tensor &w, const MaybeTensor &bias, const MaybeTensor &res, int64_t act) {
+at::Tensor fused_linear(const at::Tensor &x_, const at::Tensor &w_, const MaybeTensor &bias_, const MaybeTensor &res_, int64_t act) {
+  const at::Tensor x = turned(x_), w = turned(w_);
+  const MaybeTensor bias = turned(bias_), res = turned(res_);
   if (x.is_cuda() && at::autocast::is_autocast_enabled(at::kCUDA)) {
     const auto type = at::autocast::get_autocast_dtype(at::kCUDA);
     c10::impl::ExcludeDispatchKeyGuard off(at::autocast::get_autocast_dispatch_key_from_device_type(at::kCUDA));
@@ -299,7 +305,7 @@ struct TopkDistill : public torch::autograd::Function<TopkDistill> {
       out[0] = at::empty(logits.sizes(), logits.options());
       if (out[0].numel() > 0) {
         const Rows s(logits, classes);
-        const at::Tensor g = grads[0].to(at::kFloat).contiguous();
+        const at::Tensor g = turned(grads[0]).to(at::kFloat).contiguous();
         check_rc(obb_topk_distill_backward(ptr(s.t), s.ld, rows, classes, code_of(logits.scalar_type()), ptr(v), ptr(i), (int)v.size(-1), code_of(v.scalar_type()),
                                            (int)i.element_size(), (float)temperature, (const float *)ptr(w), (const float *)ptr(stats), (const float *)ptr(g), scale < 0 ? 1 : 0,
                                            scale < 0 ? 1.f : (float)scale, ptr(out[0]), classes, stream_of(logits)),
@@ -313,7 +319,7 @@ struct TopkDistill : public torch::autograd::Function<TopkDistill> {
 at::Tensor topk_distill(const at::Tensor &logits, const at::Tensor &values, const at::Tensor &indices, double temperature, const MaybeTensor &weight, double scale) {
   check_distill(logits, values, indices, weight);
   // (the teacher's values are a constant: cut from whatever graph they come from)
-  return TopkDistill::apply(logits, values.detach(), indices, weight, temperature, scale);
+  return TopkDistill::apply(turned(logits), turned(values.detach()), indices, turned(weight), temperature, scale);
 }
 
 }  // namespace

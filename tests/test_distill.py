@@ -425,6 +425,27 @@ def test_avg_factor_of_unreduced_losses(device, monkeypatch):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('rows, classes, k', [(1, 1, 1), (1, 9, 1), (4, 1, 1), (5, 9, 2)])
+def test_tensors_with_the_negative_bit(rows, classes, k):
+    """float tensors that are the imaginary part of a conjugate, at sizes at which they pass for contiguous ones and at others"""
+    from aidet_amd import topk_distill_loss
+
+    def pair(*shape):
+        t = torch.view_as_complex(torch.randn(*shape, 2, device=DEV)).conj().imag
+        assert t.is_neg()
+        return t, t.clone().resolve_neg()
+    torch.manual_seed(4)
+    inputs = [pair(rows, classes), pair(rows, k), pair(rows), pair(rows)]
+    indices = torch.arange(k, device=DEV).expand(rows, k).contiguous()
+    results = []
+    for logits, values, weight, up in zip(*inputs):
+        logits = logits.detach().requires_grad_(True)
+        loss = topk_distill_loss(logits, values, indices, 1., weight, 'none')
+        results.append((loss.detach(), torch.autograd.grad(loss, logits, up)[0]))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.gpu
 def test_a_head_learns_from_a_teachers_top_logits():
     """FC trunk, class logits, loss and gradients together: against the same chain in 64 bits.  Whole steps of fp32: the
     trunk's and the loss's errors (at most 1e-5 relative each at these sizes, by the tolerances of their own tests) pass

@@ -891,3 +891,26 @@ def test_capture_beside_an_eager_graph_whose_leaves_are_behind_other_nodes(way):
         torch.cuda.synchronize()
         assert torch.equal(w.grad, want)
     w.grad = None
+
+
+def lazily_negative(*shape):
+    """(a float tensor whose negative bit is set, the same numbers in memory): the imaginary part of a conjugate"""
+    t = torch.view_as_complex(torch.randn(*shape, 2, device=DEV)).conj().imag
+    assert t.is_neg()
+    return t, t.clone().resolve_neg()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('m, k, n', [(5, 1, 3), (5, 4, 1), (1, 1, 1), (6, 7, 8)])
+def test_tensors_with_the_negative_bit(m, k, n):
+    """sizes at which such a tensor passes for a contiguous one, and others; as gradients of the output too"""
+    from aidet_amd import fused_linear
+    torch.manual_seed(3)
+    pairs = [lazily_negative(*s) for s in ((m, k), (n, k), (n, ), (m, n))]
+    dy, plain_dy = lazily_negative(m, n)
+    results = []
+    for which, up in ((0, dy), (1, plain_dy)):
+        leaves = [p[which].detach().requires_grad_(True) for p in pairs]
+        y = fused_linear(*leaves, act='silu')
+        results.append([y.detach()] + list(torch.autograd.grad(y, leaves, up)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
