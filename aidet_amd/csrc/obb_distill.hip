@@ -441,14 +441,14 @@ template <typename T> static Args rows_of(const Args &a, int64_t r0, int64_t n) 
   return b;
 }
 
-template <typename T> static int forward(const Args &a, float2 *ws, hipStream_t st) {
+// (`parts`: of the whole call, as the workspace is sized for it -- the few rows that a long call may end with must not be cut)
+template <typename T> static int forward(const Args &a, int parts, float2 *ws, hipStream_t st) {
   if (a.rows > ROWS) {
     for (int64_t r0 = 0; r0 < a.rows; r0 += ROWS)
-      if (int rc = forward<T>(rows_of<T>(a, r0, a.rows - r0 < ROWS ? a.rows - r0 : ROWS), ws, st)) return rc;
+      if (int rc = forward<T>(rows_of<T>(a, r0, a.rows - r0 < ROWS ? a.rows - r0 : ROWS), parts, ws, st)) return rc;
     return OBB_OK;
   }
   if (!short_rows<T, true>(a, st)) {
-    const int parts = parts_of(a.rows, a.classes);
     if (parts == 1) {
       if (a.classes <= WAVE_ROW && a.k <= 256) distill_forward_kernel<T, 64, 256><<<(unsigned)a.rows, 64, 0, st>>>(a);
       else if (a.k <= 256) distill_forward_kernel<T, 256, 256><<<(unsigned)a.rows, 256, 0, st>>>(a);
@@ -464,14 +464,13 @@ template <typename T> static int forward(const Args &a, float2 *ws, hipStream_t 
   return OBB_OK;
 }
 
-template <typename T> static int backward(const Args &a, hipStream_t st) {
+template <typename T> static int backward(const Args &a, int parts, hipStream_t st) {
   if (a.rows > ROWS) {                                // (the last rows first, as within a launch)
     for (int64_t end = a.rows; end > 0; end -= end < ROWS ? end : ROWS)
-      if (int rc = backward<T>(rows_of<T>(a, end < ROWS ? 0 : end - ROWS, end < ROWS ? end : ROWS), st)) return rc;
+      if (int rc = backward<T>(rows_of<T>(a, end < ROWS ? 0 : end - ROWS, end < ROWS ? end : ROWS), parts, st)) return rc;
     return OBB_OK;
   }
   if (!short_rows<T, false>(a, st)) {
-    const int parts = parts_of(a.rows, a.classes);
     const int64_t per = parts == 1 ? a.classes : ((a.classes + parts - 1) / parts + 7) / 8 * 8;
     // (a grid's second dimension ends at 65535: more rows go in several launches)
     for (int64_t end = a.rows; end > 0;) {
@@ -527,7 +526,9 @@ extern "C" int obb_topk_distill_forward(const void *logits, int64_t ld, int64_t 
   a.k = k; a.vtype = vtype; a.wide_index = index_bytes == 8; a.inv_temp = 1.f / temperature; a.temp = temperature;
   a.weight = weight; a.loss = row_loss; a.stats = (float2 *)stats;
   if (rows > 0) {
-    const int rc = dtype == OBB_F32 ? forward<float>(a, (float2 *)ws, st) : dtype == OBB_BF16 ? forward<__bf16>(a, (float2 *)ws, st) : forward<_Float16>(a, (float2 *)ws, st);
+    const int parts = parts_of(rows, classes);
+    const int rc = dtype == OBB_F32 ? forward<float>(a, parts, (float2 *)ws, st)
+                 : dtype == OBB_BF16 ? forward<__bf16>(a, parts, (float2 *)ws, st) : forward<_Float16>(a, parts, (float2 *)ws, st);
     if (rc) return rc;
   }
   if (loss) {
@@ -553,5 +554,6 @@ extern "C" int obb_topk_distill_backward(const void *logits, int64_t ld, int64_t
   a.k = k; a.vtype = vtype; a.wide_index = index_bytes == 8; a.inv_temp = 1.f / temperature; a.temp = temperature;
   a.weight = weight; a.stats = (float2 *)stats; a.grad = grad; a.grad_stride = grad_stride; a.scale = scale;
   a.dlogits = dlogits; a.ldd = ldd;
-  return dtype == OBB_F32 ? backward<float>(a, st) : dtype == OBB_BF16 ? backward<__bf16>(a, st) : backward<_Float16>(a, st);
+  const int parts = parts_of(rows, classes);
+  return dtype == OBB_F32 ? backward<float>(a, parts, st) : dtype == OBB_BF16 ? backward<__bf16>(a, parts, st) : backward<_Float16>(a, parts, st);
 }

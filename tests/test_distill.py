@@ -340,6 +340,32 @@ def test_more_rows_than_a_launch_holds(rows, classes, k):
 
 
 @pytest.mark.gpu
+def test_long_rows_behind_the_last_full_launch():
+    """a call of more rows than one launch takes whose last launch has few of them, long enough to be cut into parts if they were a
+    call of their own: 137 GB of logits, losses only"""
+    from aidet_amd import topk_distill_loss
+    rows, classes = (1 << 23) + 17, 8192
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 160 << 30:
+        pytest.skip('needs 160 GB of free memory')
+    g = torch.Generator(device=DEV).manual_seed(53)
+    few = torch.randn(256, classes, generator=g, device=DEV).half()
+    logits = torch.empty(rows, classes, device=DEV, dtype=torch.float16)
+    logits[:1 << 23].view(-1, 256, classes).copy_(few)
+    logits[1 << 23:] = few[:17]
+    values, indices = few.float().topk(2, 1)
+    values, indices = values.repeat(1 << 15, 1), indices.int().repeat(1 << 15, 1)
+    values, indices = torch.cat([values, values[:17]]), torch.cat([indices, indices[:17]])
+    loss = topk_distill_loss(logits, values, indices, reduction='none')
+    del logits
+    torch.cuda.empty_cache()
+    want, _, tol, _ = reference(few, values[:256], indices[:256], 1., None)
+    for part in (loss[:1 << 23].view(-1, 256), loss[1 << 23:][None]):
+        n = part.size(1)
+        assert bool(((part.double() - want[:n]).abs() <= tol[:n]).all())
+
+
+@pytest.mark.gpu
 def test_against_differences():
     """fp32 against central differences of the plain form in 64 bits (h = 1e-5: good to ~1e-9)"""
     for rows, classes, k in ((6, 16, 4), (4, 1500, 40)):
