@@ -10,7 +10,8 @@ namespace lin {
 
 // ---- the splits of K joined: eight columns a thread, splits in order.  The loads of U splits, all of them, are under way at once
 // (one after the other their latency made 9 us of 16 splits of 24 x 1024), and few outputs go by workgroups of one wave, on more
-// CUs.  Forward, us, eight under way in workgroups of four waves and this: 24 x 12544 x 1024 fp16 13.2, 12.3; 32 x 4096 x 1024 bf16 9.6, 8.4.
+// CUs.  Forward, us, eight under way in workgroups of four waves and this: 24 x 12544 x 1024 fp16 13.4, 12.3 (weights that change from call
+// to call 14.0, 13.3), fp32 24.3, 22.8; 32 x 4096 x 1024 bf16 10.1, 8.9 (10.5 either way).
 template <typename T, int U>
 __global__ __launch_bounds__(256) void join_splits_kernel(Gemm<T> g, const float *partial, int splits, uint32_t per_row) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -117,7 +118,8 @@ int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
     rc = gemm_split<TA, TB>(g, p.tile, p.splits, ws, stream);
   } else {
     // Direct loads need 16-byte chunks that end with the operand, and a slab that fits a buffer descriptor: 256 rows, or 64
-    // where the contraction is outermost, below 2 GiB.  (4096^3 bf16: 105 us; 4095^3 through registers 250.)
+    // where the contraction is outermost, below 2 GiB.  (4096^3 bf16: forward 105 us, the
+    // gradients' products 108 and 111; 4095^3 through registers 227, 295 and 429.)
     if (aligned16(g.a, g.lda, TA ? g.m : g.k) && aligned16(g.b, g.ldb, TB ? g.n : g.k) && g.lda < (1 << 22) - 256 && g.ldb < (1 << 22) - 256)
       rc = gemm_mfma<T, TA, TB>(g, p.tile, p.splits, ws, stream);
     else
@@ -127,7 +129,9 @@ int gemm(const Gemm<T> &g, float *ws, hipStream_t stream) {
 }
 
 // ---- dz = dy act'(z) and db = sum_m dz: one pass over dy, column sums in two fixed steps (no atomics: the same bits
-// every run).  dz is rounded to the type once, as the two products take operands of the type; db sums what was not rounded.
+// every run).  dz is rounded to the type once, as the two products take operands of the type; db sums what was not rounded.  For 16-bit types
+// with gelu or silu that is half the error of dx and dW: their rms is 1.41 times what an fp32 dz would leave (bf16 0.00235 and
+// 0.00166 relative, fp16 0.00029 and 0.00021); a dz of two 16-bit parts would be products of twice the length.  (relu: dy or 0, exact.)
 // Block (x, y): 64 columns, rows y, y + chunks, ... of a few dozen; 16-byte accesses, four rows under way a thread, or one where
 // four would leave the device short of workgroups (both kernels, us, four and one: 777 x 515 fp32 gelu 10.6, 7.6; 1024 x 1024
 // bf16 relu 7.7, 7.0); partial sums [chunk][n] in the workspace.  Larger ones are memory's: 8192 x 1024 fp32 silu 24.8 us = 4.1 TB/s, gelu 26.7.

@@ -6,8 +6,8 @@
 // matrix instructions.  One barrier a slab, in its middle: when everybody has the second half's fragments, the slab's slots
 // are free for loads that are due a slab later.  A wave issues in order, so loads, LDS reads and matrix instructions are dealt
 // evenly by hand: eight loads in a row held the matrix pipe back (4096 x 16384 x 4096: 427 us, dealt 402).
-// What bounds it: at 8192 x 4096 x 16384 (895 us with relu = 1228 TFLOP/s) the matrix pipe is busy 64 % at 1.9 GHz; without the
-// loads 727 us, without the matrix instructions 680: the slabs' latency behind L2 (79 % hits) is not all covered, and
+// What bounds it: at 8192 x 4096 x 16384 (895 us with gelu = 1228 TFLOP/s) the matrix pipe is busy 55 % at 2.07 GHz; without the
+// loads 727 us, without the matrix instructions 680: the slabs' latency behind L2 (81 % hits) is not all covered, and
 // every round of tiles begins and ends with an idle matrix pipe (about 10 us of 110).  Tried: slots of 32 k, five deep (rows
 // of 64 bytes double the L2 requests: 957 us), 32 x 32 instructions (1010), four waves of 128 x 128 (1000), raised priority
 // around the matrix instructions (930).

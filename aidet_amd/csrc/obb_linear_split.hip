@@ -10,8 +10,9 @@
 // Where a part or a sum overflows -- |x| from 2^112 on, infinite ones too, products and sums from 2^96 on -- the sum is infinite or a
 // NaN.  A workgroup that finds such sums computes those again with the fp32 matrix instruction, whose range, infinities and
 // NaNs are IEEE's.
-// What bounds it: 4096^3 615 us = 224 TFLOP/s (597 without the two multiplications a pair; the fp32 matrix instruction's library product: 154), matrix pipe busy 66 % at
-// 1.96 GHz; the rest is splitting (two vector instructions a matrix instruction) and the two barriers of a step.
+// What bounds it: 4096^3 615 us = 224 TFLOP/s (597 without the two multiplications a pair; the fp32 matrix instruction's library
+// product: 154), matrix pipe busy 59 % at 2.05 GHz (652 us under the counters); the rest is splitting (2.3 vector instructions a matrix
+// instruction) and the two barriers of a step.
 #include "obb_linear_internal.h"
 
 namespace obb {
